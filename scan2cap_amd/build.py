@@ -20,6 +20,10 @@ HIPCC_FLAGS = [
     # hardware float atomics (global_atomic_add_f32) instead of CAS loops in the
     # scatter-add (grad) kernels
     "-munsafe-fp-atomics",
+    # no packed-fp32 instructions (v_pk_add / mul / fma_f32): some of their forms have given wrong
+    # results on this hardware; the scalar forms round the same (hipcc's host pass warns that it does
+    # not know the feature -- harmless)
+    "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     "-fPIC",
 ]
 OBJ_DIR = os.path.join(LIB_DIR, "obj")
