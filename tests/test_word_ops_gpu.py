@@ -1,0 +1,639 @@
+"""scan2cap_amd.word_ops against their definitions in float64.
+
+Tolerances.  u = 2^-24.  A logit difference d = (x - m) / T in base 2 carries at most 6 u |d| (the
+difference, the factor's three roundings, the product, the power of two), a sum of positive terms over V
+words at most one rounding per addition of a lane's chain (V / 64 additions at most) and 20 for the joins,
+and the terms' own errors enter a softmax sum weighted by p: sum p |d| <= log2 V + 1 < 20.  So a log
+probability is off by at most u (6 |log p| / ln 2 + V / 64 + 20 + 6 * 20).  The entropy's second sum carries
+p |d| (8 + 6 |d|) u with sum p d^2 < 20^2, on top of that.  A gradient is p (A + B d) + entries: p's relative
+error is ln 2 times that of log2 p, d at most 160; 16-bit results add half a step, finfo.eps / 2."""
+import math
+
+import pytest
+import torch
+
+from scan2cap_amd import word_ops
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+NAN, INF = float("nan"), float("inf")
+TYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def _log_tol(V, logp):
+    return U * (9 * logp.abs() + V / 64 + 140)
+
+
+def _step(t):
+    """half a step of the type, relative, and its smallest half step"""
+    f = torch.finfo(t)
+    return f.eps / 2, f.tiny * f.eps if t != torch.float32 else 2.0 ** -126
+
+
+def _logits(shape, V, dtype, seed, spread=3.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(tuple(shape) + (V,), generator=g, device="cuda") * spread).to(dtype)
+
+
+def _ints(shape, hi, seed, lo=0):
+    g = torch.Generator(device="cuda").manual_seed(seed + 1000)
+    return torch.randint(lo, hi, tuple(shape), generator=g, device="cuda")
+
+
+def _randn(shape, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed + 2000)
+    return torch.randn(tuple(shape), generator=g, device="cuda")
+
+
+def _scores64(x, tokens, k, T, ignore=None):
+    """-> logp, entropy, log p, p, ids by the definition; rows of all -inf: log p = -inf, p = 0."""
+    z = x.double() / T
+    m = z.amax(-1, keepdim=True)
+    m = torch.where(m == -INF, torch.zeros_like(m), m)
+    e = torch.exp(z - m)
+    s = e.sum(-1, keepdim=True)
+    empty = s == 0
+    lq = (z - m) - torch.log(torch.where(empty, torch.ones_like(s), s))
+    p = e / torch.where(empty, torch.ones_like(s), s)
+    h = -torch.where(p == 0, torch.zeros_like(p), p * lq).sum(-1)
+    logp = None
+    if tokens is not None:
+        bad = (tokens < 0) | (tokens >= x.shape[-1])
+        logp = lq.gather(-1, tokens.clamp(0, x.shape[-1] - 1).unsqueeze(-1)).squeeze(-1)
+        logp = torch.where(bad, torch.full_like(logp, NAN), logp)
+    ids = torch.sort(x.double() + 0.0, dim=-1, descending=True, stable=True)[1][..., :k]
+    return logp, h, lq, p, ids
+
+
+def _scores_grad64(x, tokens, ids, lq, p, h, T, gl, ge, gt):
+    g = torch.zeros_like(p)
+    if gl is not None:
+        g.scatter_add_(-1, tokens.unsqueeze(-1), gl.double().unsqueeze(-1))
+    if gt is not None:
+        g.scatter_add_(-1, ids, gt.double())
+    total = g.sum(-1, keepdim=True)
+    if ge is not None:
+        total = total + ge.double().unsqueeze(-1) * (torch.where(p == 0, torch.zeros_like(p), lq) + h.unsqueeze(-1))
+    return (g - p * total) / T
+
+
+def _grad_tol(dtype, ref, V, p, lq, T, amount):
+    """amount: the sum of the upstream gradients' sizes, (...)."""
+    half, tiny = _step(dtype)
+    d = torch.where(p == 0, torch.zeros_like(p), lq.abs())
+    rel = U * (9 * d + V / 64 + 160)
+    return ref.abs() * half + tiny + (amount.double().unsqueeze(-1) / T) * (p * (rel * (1 + d + 20) + U * (d + 20)) + 8 * U)
+
+
+def _check_scores(x, tokens, k=0, T=1.0, ignore=None, grads="let", seed=0):
+    V = x.shape[-1]
+    leaf = x.detach().requires_grad_()
+    out = word_ops.token_scores(leaf, tokens, top_k=k, temperature=T, ignore_index=ignore)
+    logp, h, lq, p, ids = _scores64(x, tokens, k, T)
+    live = torch.ones_like(h, dtype=torch.bool) if ignore is None else tokens != ignore
+    zero = torch.zeros_like(h)
+
+    def close(a, b, tol, what):
+        b, tol = b.expand_as(a), tol.expand_as(a)
+        same = (a.double() == b) | (a.isnan() & b.isnan()) | ((a.double() - b).abs() <= tol)
+        assert bool(same.all()), (what, float((a.double() - b).abs().nan_to_num().max()), a.shape)
+
+    if tokens is not None:
+        want = torch.where(live, logp, zero)
+        close(out.logp, want, _log_tol(V, want.nan_to_num(0, 0, 0)), "logp")
+    want = torch.where(live, h, zero)
+    close(out.entropy, want, torch.full_like(want, U * (4000 + V / 64 * 20)), "entropy")
+    if k:
+        assert torch.equal(out.top_ids, torch.where(live.unsqueeze(-1), ids, torch.full_like(ids, -1)))
+        want = torch.where(live.unsqueeze(-1), lq.gather(-1, ids), zero.unsqueeze(-1))
+        close(out.top_logp, want, _log_tol(V, want.nan_to_num(0, 0, 0)), "top_logp")
+    gl = _randn(h.shape, seed) if "l" in grads and tokens is not None else None
+    ge = _randn(h.shape, seed + 1) if "e" in grads else None
+    gt = _randn(h.shape + (k,), seed + 2) if "t" in grads and k else None
+    pairs = [(o, g) for o, g in ((out.logp, gl), (out.entropy, ge), (out.top_logp, gt)) if g is not None]
+    if pairs:
+        dx, = torch.autograd.grad([a for a, _ in pairs], [leaf], [b for _, b in pairs])
+        assert dx.dtype == x.dtype and dx.shape == x.shape
+        safe = tokens.clamp(0, V - 1) if tokens is not None else None
+        ref = _scores_grad64(x, safe, ids, lq, p, h, T, gl, ge, gt)
+        dead = ~live | (p.sum(-1) == 0)
+        ref = torch.where(dead.unsqueeze(-1), torch.zeros_like(ref), ref)
+        if tokens is not None:
+            bad = live & ~dead & ((tokens < 0) | (tokens >= V))
+            ref = torch.where(bad.unsqueeze(-1), torch.full_like(ref, NAN), ref)
+        amount = sum(g.abs() if g.dim() == h.dim() else g.abs().sum(-1) for _, g in pairs)
+        close(dx, ref, _grad_tol(x.dtype, ref.nan_to_num(), V, p.nan_to_num(), lq.nan_to_num(0, 0, 0), T, amount), "dx")
+    return out
+
+
+SIZES = [(1, 1, 1), (2, 2, 2), (3, 3, 1), (5, 63, 5), (4, 64, 64), (3, 65, 64), (7, 255, 20), (2, 257, 3),
+         (3, 1000, 33), (2, 1023, 64), (2, 1025, 1), (5, 3500, 5), (2, 4097, 64), (3, 16385, 17),
+         (2, 50001, 20), (1, 131072, 8), (1, 262143, 64), (300, 300, 5), (5000, 37, 3)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,V,k", SIZES)
+def test_scores_over_sizes(rows, V, k, dtype):
+    x = _logits((rows,), V, dtype, rows + V)
+    _check_scores(x, _ints((rows,), V, V), k, T=1.0, seed=V)
+
+
+@pytest.mark.parametrize("T", [0.05, 0.7, 2.0, 100.0])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_scores_temperature(dtype, T):
+    x = _logits((6,), 3500, dtype, 3)
+    _check_scores(x, _ints((6,), 3500, 4), 7, T=T)
+
+
+@pytest.mark.parametrize("grads", ["l", "e", "t", "le", "lt", "et"])
+def test_scores_each_gradient_alone(grads):
+    x = _logits((6,), 777, torch.float32, 5)
+    t = _ints((6,), 777, 6)
+    _check_scores(x, t, 5, T=1.5, grads=grads)
+    # the scored word among the alternatives, and without tokens
+    _check_scores(x, x.argmax(-1), 5, grads=grads)
+    if "l" not in grads:
+        _check_scores(x, None, 5, grads=grads)
+
+
+def test_scores_gradient_against_differences():
+    """Central differences of the float64 definition along random directions."""
+    x = _logits((4,), 501, torch.float32, 8)
+    t, k, T = _ints((4,), 501, 9), 6, 1.3
+    leaf = x.clone().requires_grad_()
+    out = word_ops.token_scores(leaf, t, top_k=k, temperature=T)
+    w = [_randn((4,), 1), _randn((4,), 2), _randn((4, k), 3)]
+    dx, = torch.autograd.grad(out[:3], [leaf], w)
+
+    def f(z):
+        logp, h, lq, _, _ = _scores64(z, t, k, T)
+        return (logp * w[0] + h * w[1] + (lq.gather(-1, out.top_ids) * w[2]).sum(-1)).sum()
+    for s in range(4):
+        v = _randn(x.shape, 10 + s).double()
+        h = 1e-4
+        want = (f(x.double() + h * v) - f(x.double() - h * v)) / (2 * h)
+        # the kernel's rounding (1e-5 of the sum of sizes) and the differences' own h^2 term
+        assert abs(float((dx.double() * v).sum() - want)) <= 1e-5 * float((dx.double() * v).abs().sum()) + 1e-5
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_scores_masked_words_and_rows(dtype):
+    V, low = 1500, torch.finfo(dtype).min
+    x = _logits((10,), V, dtype, 11)
+    x[0, ::2] = -INF
+    x[1, 1:] = -INF                       # one word left
+    x[2] = -INF                           # none
+    x[3, :-1] = low
+    x[4] = low                            # nothing but the lowest value: uniform
+    x[5, 700:] = -INF
+    x[6] = 2.5                            # all equal: lowest indices first
+    x[7] = torch.arange(V, device="cuda").to(dtype) / 256       # ascending: every tile beats the last
+    x[8] = -torch.arange(V, device="cuda").to(dtype) / 256
+    x[9] = (torch.arange(V, device="cuda") % 5).to(dtype)
+    x[9, ::5] = -0.0
+    t = torch.tensor([1, 0, 3, V - 1, 7, 800, 0, V - 1, 0, 5], device="cuda")
+    for k in (0, 1, 9, 64):
+        _check_scores(x, t, k)
+    t[0] = 2                              # a word that cannot be said: logp -inf
+    out = word_ops.token_scores(x, t)
+    assert out.logp[0].item() == -INF and out.logp[2].item() == -INF and out.entropy[2].item() == 0
+
+
+def test_scores_signed_zeros_tie():
+    x = torch.full((1, 300), -1.0, device="cuda")
+    x[0, 5], x[0, 17], x[0, 90] = -0.0, 0.0, -0.0
+    out = word_ops.token_scores(x, None, top_k=4)
+    assert out.top_ids[0].tolist() == [5, 17, 90, 0]
+
+
+@pytest.mark.parametrize("V", [37, 3500, 70000])
+@pytest.mark.parametrize("value", [NAN, INF])
+def test_scores_nan_and_inf(V, value):
+    """They stay in their row, and in an ignored row leave no trace."""
+    x = _logits((4,), V, torch.float32, 12)
+    x[1, V // 3] = value
+    x[3, V - 1] = value
+    t = torch.tensor([5, 6, 7, 0], device="cuda")
+    leaf = x.clone().requires_grad_()
+    out = word_ops.token_scores(leaf, t, top_k=3, ignore_index=0)
+    assert out.logp[1].isnan() and out.entropy[1].isnan() and out.top_logp[1].isnan().all()
+    assert out.top_ids[1, 0].item() == V // 3
+    assert out.logp[3].item() == 0 and out.entropy[3].item() == 0
+    assert out.top_ids[3].tolist() == [-1] * 3 and out.top_logp[3].tolist() == [0.0] * 3
+    dx, = torch.autograd.grad([out.logp, out.entropy], [leaf], [torch.ones(4, device="cuda")] * 2)
+    assert dx[1].isnan().all() and bool((dx[3] == 0).all())
+    assert dx[0].isfinite().all() and dx[2].isfinite().all() and out.logp[[0, 2]].isfinite().all()
+
+
+def test_scores_bad_tokens_and_ignored_rows():
+    x = _logits((6,), 400, torch.float32, 13)
+    t = torch.tensor([-1, 400, 2 ** 40, 3, -100, 399], device="cuda")
+    out = _check_scores(x, t, 4, ignore=-100)
+    assert out.logp.isnan().tolist() == [True, True, True, False, False, False]
+    _check_scores(x, torch.zeros(6, dtype=torch.int64, device="cuda"), 4, ignore=0)      # all ignored
+    _check_scores(x, t.clamp(0, 399).int(), 4)
+    # an ignore_index that no word has
+    _check_scores(x, t.clamp(0, 399), 4, ignore=2 ** 50)
+
+
+def _views(V, dtype):
+    base = _logits((3, 4, 5), V + 3, dtype, 14)
+    yield "offset", base[..., 1:V + 1]
+    yield "offset rows", base[1:, :, 2:, 3:]
+    yield "permuted", base[..., :V].permute(1, 2, 0, 3)
+    yield "sliced", base[:, ::2, ::3, :V]
+    yield "expanded", base[:, :1, :, :V].expand(3, 4, 5, V)
+    yield "strided words", base[..., :V + 3:2]
+    yield "five axes", _logits((2, 3, 2, 3, 2), V, dtype, 15).permute(4, 2, 0, 3, 1, 5)
+    yield "one row", base[0, 0, 0, :V]
+    yield "transposed storage", base[0, 0].t()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("V", [7, 130, 1029])
+def test_scores_strides(V, dtype):
+    for name, x in _views(V, dtype):
+        n = x.shape[-1]
+        _check_scores(x, _ints(x.shape[:-1], n, 16), min(5, n), T=0.9, seed=17)
+
+
+@pytest.mark.parametrize("shape", [(0,), (3, 0), (0, 2, 4)])
+def test_empty_batches(shape):
+    x = torch.empty(shape + (9,), device="cuda", requires_grad=True)
+    t = torch.empty(shape, dtype=torch.int64, device="cuda")
+    out = word_ops.token_scores(x, t, top_k=2)
+    assert out.logp.shape == shape and out.top_ids.shape == shape + (2,)
+    loss = word_ops.distill_loss(x, t.unsqueeze(-1).expand(shape + (3,)), x.detach()[..., :3])
+    assert loss.shape == shape
+    dx, = torch.autograd.grad([out.logp.sum() + out.entropy.sum() + loss.sum()], [x])
+    assert dx.shape == x.shape
+    table = torch.ones(4, 6, device="cuda", requires_grad=True)
+    y = word_ops.embed_tokens(t, table)
+    assert y.shape == shape + (6,)
+    g, = torch.autograd.grad([y.sum()], [table])
+    assert bool((g == 0).all())
+
+
+# ---- distillation ----------------------------------------------------------------------------------------
+def _distill64(x, ids, teacher, T, mask=None):
+    z = x.double() / T
+    V = x.shape[-1]
+    m = z.amax(-1, keepdim=True)
+    m = torch.where(m == -INF, torch.zeros_like(m), m)
+    e = torch.exp(z - m)
+    s = e.sum(-1, keepdim=True)
+    one = torch.ones_like(s)
+    lp = (z - m) - torch.log(torch.where(s == 0, one, s))
+    p = e / torch.where(s == 0, one, s)
+    w = torch.where(ids >= 0, teacher.double() / T, torch.full_like(teacher.double(), -INF))
+    wm = w.amax(-1, keepdim=True)
+    wm = torch.where(wm == -INF, torch.zeros_like(wm), wm)
+    ew = torch.exp(w - wm)
+    sw = ew.sum(-1, keepdim=True)
+    dead = (sw == 0).squeeze(-1)
+    q = ew / torch.where(sw == 0, torch.ones_like(sw), sw)
+    if mask is not None:
+        dead = dead | ~mask
+    q = torch.where(dead.unsqueeze(-1), torch.zeros_like(q), q)
+    at = lp.gather(-1, ids.clamp(0, V - 1))
+    terms = torch.where(q == 0, torch.zeros_like(q), q * ((w - wm) - torch.log(sw) - at))
+    bad = ((q != 0) & (ids >= V)).any(-1)
+    loss = torch.where(bad, torch.full_like(terms[..., 0], NAN), terms.sum(-1))
+    return torch.where(dead, torch.zeros_like(loss), loss), q, p, lp, dead, bad, at
+
+
+def _check_distill(x, ids, teacher, T=1.0, mask=None, seed=0):
+    V = x.shape[-1]
+    leaf = x.detach().requires_grad_()
+    loss = word_ops.distill_loss(leaf, ids, teacher, temperature=T, mask=mask)
+    want, q, p, lp, dead, bad, at = _distill64(x, ids.long(), teacher, T, mask)
+    size = torch.where(q == 0, torch.zeros_like(q), q * (at.abs() + q.clamp(min=1e-300).log().abs()))
+    size = size.nan_to_num(0, 0, 0).sum(-1)
+    tol = U * (10 * size + V / 64 + 300 + ids.shape[-1])
+    a = loss.double()
+    ok = (a == want) | (a.isnan() & want.isnan()) | ((a - want).abs() <= tol)
+    assert bool(ok.all()), float((a - want).abs().nan_to_num().max())
+    g = _randn(loss.shape, seed)
+    dx, = torch.autograd.grad([loss], [leaf], [g])
+    assert dx.dtype == x.dtype
+    ref = p * q.sum(-1, keepdim=True)
+    ref = ref.scatter_add(-1, ids.long().clamp(0, V - 1), -q)
+    ref = ref * (g.double() / T).unsqueeze(-1)
+    none = dead | (p.sum(-1) == 0)
+    ref = torch.where(none.unsqueeze(-1), torch.zeros_like(ref), ref)
+    ref = torch.where((bad & ~none).unsqueeze(-1), torch.full_like(ref, NAN), ref)
+    half, tiny = _step(x.dtype)
+    rel = U * (9 * torch.where(p == 0, torch.zeros_like(p), lp.abs()) + V / 64 + 160 + ids.shape[-1])
+    tol = ref.abs() * half + tiny + (g.double().abs() / T).unsqueeze(-1) * (p * rel + 200 * U)
+    b = dx.double()
+    ok = (b == ref) | (b.isnan() & ref.isnan()) | ((b - ref).abs() <= tol)
+    assert bool(ok.all()), float((b - ref).abs().nan_to_num().max())
+    return loss
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,V,K", [(1, 1, 1), (3, 2, 2), (4, 65, 64), (5, 300, 65), (2, 1025, 256),
+                                      (6, 3500, 16), (3, 4099, 33), (2, 50001, 128), (1, 262143, 7),
+                                      (5000, 41, 3)])
+def test_distill_over_sizes(rows, V, K, dtype):
+    x = _logits((rows,), V, dtype, V)
+    ids = _ints((rows, K), V, K)                       # repeated words among them
+    for T in (1.0, 2.0):
+        _check_distill(x, ids, _randn((rows, K), V).to(dtype) * 3, T, seed=K)
+
+
+@pytest.mark.parametrize("td", TYPES)
+def test_distill_teacher_type_is_its_own(td):
+    x = _logits((5,), 901, torch.bfloat16, 21)
+    _check_distill(x, _ints((5, 12), 901, 22).int(), _randn((5, 12), 23).to(td))
+
+
+def test_distill_empty_slots_rows_and_masks():
+    V, K = 640, 9
+    x = _logits((12,), V, torch.float32, 24)
+    ids = _ints((12, K), V, 25)
+    w = _randn((12, K), 26)
+    ids[0] = -1                                        # no slot at all
+    ids[1, 3:] = -7
+    ids[2] = 11                                        # one word in every slot
+    w[3] = -INF                                        # no slot with weight
+    w[4, ::2] = -INF
+    ids[5, 2], w[5, 2] = -1, NAN                       # NaN in an empty slot
+    w[6] = torch.finfo(torch.float32).min              # uniform
+    w[7, 1:] = torch.finfo(torch.float32).min
+    ids[8, 4] = V                                      # out of the vocabulary
+    ids[9, 4], w[9, 4] = 2 ** 40, -INF                 # ... in an empty slot
+    x[10] = -INF                                       # a student that can say nothing
+    x[11, ids[11, 0]] = -INF                           # ... or not what the teacher says
+    loss = _check_distill(x, ids, w)
+    assert loss[0].item() == 0 and loss[3].item() == 0 and loss[8].isnan()
+    assert loss[10].item() == INF and loss[11].item() == INF and loss[5].isfinite() and loss[9].isfinite()
+    mask = torch.arange(12, device="cuda") % 2 == 0
+    x[1] = NAN                                         # masked: not looked at
+    x[3, 5] = INF
+    loss = _check_distill(x, ids, w, mask=mask)
+    assert bool((loss[1::2] == 0).all())
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_distill_strides(dtype):
+    for name, x in _views(130, dtype):
+        ids = _ints(tuple(x.shape[:-1]) + (4,), x.shape[-1], 27)
+        t = _randn(ids.shape[::-1], 28).permute(*range(ids.dim())[::-1])          # strided teacher
+        _check_distill(x, ids, t, 1.5)
+
+
+def test_distill_from_a_teachers_alternatives():
+    """token_scores of the teacher -> distill_loss of the student: the teacher itself has loss 0 where all
+    of its words are slots, and ignored rows arrive as empty slots."""
+    V = 60
+    teacher = _logits((7,), V, torch.float32, 30)
+    t = _ints((7,), V, 31, lo=1)
+    t[2] = 0
+    best = word_ops.token_scores(teacher, t, top_k=V, temperature=2.0, ignore_index=0)
+    loss = word_ops.distill_loss(teacher * 2.0, best.top_ids, best.top_logp * 2.0, temperature=2.0)
+    # q = p at T = 2 would need teacher / 2 = (2 teacher) / 2 ... compare with the definition instead
+    want = _distill64(teacher * 2.0, best.top_ids, best.top_logp * 2.0, 2.0)[0]
+    assert bool(((loss.double() - want).abs() <= U * 500).all()) and loss[2].item() == 0
+    same = word_ops.distill_loss(teacher, best.top_ids, best.top_logp * 2.0, temperature=2.0)
+    assert bool((same.abs() <= U * 500).all())
+
+
+# ---- embedding -------------------------------------------------------------------------------------------
+def _check_embed(tokens, table, scale=1.0, pad=None, g=None, seed=0):
+    V, D = table.shape
+    leaf = table.detach().requires_grad_()
+    out = word_ops.embed_tokens(tokens, leaf, scale=scale, padding_idx=pad)
+    t = tokens.long()
+    is_pad = torch.zeros_like(t, dtype=torch.bool) if pad is None else t == pad
+    bad = ~is_pad & ((t < 0) | (t >= V))
+    fs = float(torch.tensor(scale, dtype=torch.float32))
+    want = table.double()[t.clamp(0, V - 1)] * fs
+    want = torch.where(is_pad.unsqueeze(-1), torch.zeros_like(want), want)
+    want = torch.where(bad.unsqueeze(-1), torch.full_like(want, NAN), want)
+    half, tiny = _step(table.dtype)
+    a = out.double()
+    ok = (a == want) | (a.isnan() & want.isnan()) | ((a - want).abs() <= want.abs() * (half + 2 * U) + tiny)
+    assert bool(ok.all())
+    if g is None:
+        g = _randn(out.shape, seed).to(table.dtype)
+    d, = torch.autograd.grad([out], [leaf], [g])
+    again, = torch.autograd.grad([word_ops.embed_tokens(tokens, leaf, scale=scale, padding_idx=pad)], [leaf], [g])
+    assert torch.equal(d, again) and d.dtype == table.dtype and d.shape == table.shape
+    rows = torch.where(is_pad | bad, torch.full_like(t, V), t).reshape(-1)
+    acc = torch.zeros(V + 1, D, dtype=torch.float64, device="cuda")
+    acc.index_add_(0, rows, g.double().reshape(-1, D))
+    size = torch.zeros_like(acc).index_add_(0, rows, g.double().abs().reshape(-1, D))
+    count = torch.bincount(rows, minlength=V + 1).unsqueeze(-1)
+    ref, size, count = (acc * fs)[:V], (size * abs(fs))[:V], count[:V]
+    # one rounding per addition and one for the scale, then half a step
+    tol = (count + 1) * U * size + ref.abs() * half + tiny
+    assert bool(((d.double() - ref).abs() <= tol).all()), float((d.double() - ref).abs().max())
+    assert bool((d[(count == 0).squeeze(-1)] == 0).all())
+    return out, d
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("N,V,D", [(1, 1, 1), (1, 5, 3), (7, 3, 8), (65, 10, 300), (256, 3500, 300), (1000, 97, 515),
+                                   (2048, 64, 64), (2049, 64, 64), (4096, 3500, 33), (8191, 1001, 40),
+                                   (8193, 513, 24), (20000, 70000, 16), (70001, 257, 9), (300, 5, 4099),
+                                   (100000, 1, 8), (9000, 131072, 4)])
+def test_embed_over_sizes(N, V, D, dtype):
+    _check_embed(_ints((N,), V, N), _logits((V,), D, dtype, V, 1.0), scale=1.7, seed=D)
+
+
+@pytest.mark.parametrize("N", [1, 500, 30000])
+def test_embed_padding_and_bad_tokens(N):
+    V = 50
+    t = _ints((N,), V + 3, 41, lo=-3)
+    table = _logits((V,), 20, torch.float32, 42, 1.0)
+    for pad in (None, 0, 49, -3, 52, 10 ** 12):
+        _check_embed(t, table, 0.5, pad)
+    _check_embed(torch.full((N,), 7, device="cuda"), table, 2.0, 7)              # nothing but padding
+    _check_embed(torch.full((N,), 2 ** 40 + 3, device="cuda"), table, 2.0, 7)    # nothing but bad ones
+    _check_embed(torch.full((N,), 7, device="cuda"), table, 2.0)                 # one word
+
+
+def test_embed_one_word_takes_most_places():
+    t = _ints((40000,), 300, 43)
+    t[_ints((30000,), 40000, 44)] = 2
+    for D, dtype in ((7, torch.float32), (1030, torch.bfloat16)):
+        _check_embed(t, _logits((300,), D, dtype, 45, 1.0), 1.0, 0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_embed_strides(dtype):
+    big = _logits((40,), 70, dtype, 46, 1.0)
+    t = _ints((6, 5, 4), 40, 47)
+    _check_embed(t, big[:, 3:64])                          # a slice of a wider table
+    _check_embed(t.permute(2, 0, 1), big[::2][:, 1:])      # even rows; the higher tokens are bad ones
+    _check_embed(t[:, ::2].int(), big)
+    _check_embed(t[0, 0, 0], big)
+    table = big[:, :64]
+    g = _randn((6, 5, 4, 130), 48).to(dtype)
+    _check_embed(t, table, g=g[..., 1:65])                 # strided rows of the gradient
+    _check_embed(t, table, g=g[..., :128:2])
+    _check_embed(t, table, g=g[:, :, :1, :64].expand(6, 5, 4, 64))
+    _check_embed(t, table, g=g[:1, :1, :1, :1].expand(6, 5, 4, 64))
+    _check_embed(t, table, g=_randn((64, 4, 5, 6), 49).to(dtype).permute(3, 2, 1, 0))
+
+
+def test_embed_gradient_against_differences():
+    table = _logits((30,), 11, torch.float32, 50, 1.0)
+    t = _ints((70,), 30, 51)
+    leaf = table.clone().requires_grad_()
+    w = _randn((70, 11), 52)
+    d, = torch.autograd.grad([word_ops.embed_tokens(t, leaf, 3.0, 4)], [leaf], [w])
+    v = _randn((30, 11), 53)
+    f = lambda z: (z.double()[t] * 3.0 * (t != 4).unsqueeze(-1) * w.double()).sum()     # noqa: E731
+    h = 1e-3
+    want = float((f(table.double() + h * v.double()) - f(table.double() - h * v.double())) / (2 * h))
+    # linear in the table: the kernel's sums of at most 70 terms, and 1e-10 for the quotient
+    assert abs(float((d.double() * v.double()).sum()) - want) <= 72 * U * float((d * v).abs().sum()) * 3 + 1e-8
+
+
+# ---- streams, graphs, sizes past 32 bits --------------------------------------------------------------------
+def _pipeline(table, W, tokens, target, teacher):
+    """embed -> product -> scores and distillation, as a training step runs them together."""
+    h = word_ops.embed_tokens(tokens, table, scale=2.0, padding_idx=0)
+    logits = torch.tanh(h) @ W
+    best = word_ops.token_scores(teacher, target, top_k=6, temperature=1.5, ignore_index=0)
+    sc = word_ops.token_scores(logits, target, top_k=3, ignore_index=0)
+    kd = word_ops.distill_loss(logits, best.top_ids, best.top_logp * 1.5, temperature=1.5,
+                               mask=target != 0)
+    loss = (-sc.logp - 0.01 * sc.entropy + 0.5 * kd).sum() / target.numel()
+    return (loss,) + torch.autograd.grad([loss], [table, W])
+
+
+def _pipeline_inputs(seed):
+    V, E = 350, 24
+    table = (_randn((V, E), seed) * 0.3).requires_grad_()
+    W = (_randn((E, V), seed + 1) * 0.5).requires_grad_()
+    tokens, target = _ints((5, 9), V, seed), _ints((5, 9), V, seed + 3)
+    target[:, 6:] = 0
+    return table, W, tokens, target, _randn((5, 9, V), seed + 4) * 2
+
+
+def test_operators_together():
+    """The three in one step against the same step in float64 autograd."""
+    table, W, tokens, target, teacher = _pipeline_inputs(60)
+    loss, dt, dW = _pipeline(table, W, tokens, target, teacher)
+    t64, W64 = table.detach().double().requires_grad_(), W.detach().double().requires_grad_()
+    logits = torch.tanh(t64[tokens] * 2.0 * (tokens != 0).unsqueeze(-1)) @ W64
+    lq = torch.log_softmax(logits, -1)
+    live = (target != 0).double()
+    logp = lq.gather(-1, target.unsqueeze(-1)).squeeze(-1)
+    H = -(lq.exp() * lq).sum(-1)
+    top, ids = torch.topk(teacher.double(), 6, dim=-1)
+    q = torch.softmax(top / 1.5, -1)
+    kd = (q * (q.log() - torch.log_softmax(logits / 1.5, -1).gather(-1, ids))).sum(-1)
+    want = ((-logp - 0.01 * H + 0.5 * kd) * live).sum() / target.numel()
+    wt, wW = torch.autograd.grad([want], [t64, W64])
+    # float32 products of 24 and 350 terms in between: 1e-5 of the largest entry
+    assert abs(float(loss.detach()) - float(want.detach())) <= 1e-5 * abs(float(want.detach()))
+    assert float((dt.double() - wt).abs().max()) <= 1e-5 * float(wt.abs().max())
+    assert float((dW.double() - wW).abs().max()) <= 1e-5 * float(wW.abs().max())
+
+
+def test_on_another_stream():
+    ins = _pipeline_inputs(61)
+    want = _pipeline(*ins)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = _pipeline(*ins)
+        other = _pipeline(*ins)
+    side.synchronize()
+    for a, b, c in zip(want, got, other):
+        assert torch.equal(a, b) and torch.equal(a, c)
+
+
+def test_captured_and_replayed():
+    """Two graphs in one pool over the same inputs, replayed in turn with eager work between; every
+    replay against the eager result for that replay's inputs."""
+    def step(x, t, ids, w, table, up):
+        leaf = x.detach().requires_grad_()
+        tab = table.detach().requires_grad_()
+        sc = word_ops.token_scores(leaf, t, top_k=4, temperature=1.2, ignore_index=0)
+        kd = word_ops.distill_loss(leaf, ids, w, temperature=2.0)
+        y = word_ops.embed_tokens(t, tab, scale=0.5, padding_idx=0)
+        return [sc.logp, sc.entropy, sc.top_logp, sc.top_ids, kd, y] + list(torch.autograd.grad(
+            [sc.logp, sc.entropy, kd, y], [leaf, tab], [up[:, 0], up[:, 1], up[:, 2], up[:, 3:]]))
+
+    def inputs(rows, V, seed):
+        return [_logits((rows,), V, torch.float32, seed), _ints((rows,), V, seed), _ints((rows, 7), V, seed + 1),
+                _randn((rows, 7), seed), _randn((V, 6), seed + 2), _randn((rows, 9), seed + 3)]
+    cases = [(20, 513), (2, 70001), (9000, 40)]
+    for rows, V in cases:
+        static = inputs(rows, V, 70)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step(*static)
+        torch.cuda.current_stream().wait_stream(side)
+        graphs, pool = [], None
+        for _ in range(2):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, pool=pool):
+                out = step(*static)
+            pool = g.pool()
+            graphs.append((g, out))
+        for it in range(4):
+            new = inputs(rows, V, 80 + it)
+            for a, b in zip(static, new):
+                a.copy_(b)
+            g, out = graphs[it % 2]
+            g.replay()
+            got = [o.clone() for o in out]
+            want = step(*new)
+            torch.cuda.synchronize()
+            for i, (a, b) in enumerate(zip(got, want)):
+                assert torch.equal(a, b), (rows, V, it, i)
+
+
+def test_rows_past_32_bit_offsets():
+    rows, V = 70000, 32768                     # 2.3e9 elements
+    x = torch.zeros(rows, V, dtype=torch.bfloat16, device="cuda")
+    x[-3:] = _logits((3,), V, torch.bfloat16, 90)
+    t = torch.zeros(rows, dtype=torch.int64, device="cuda")
+    t[-3:] = _ints((3,), V, 91, lo=1)
+    leaf = x.requires_grad_()
+    out = word_ops.token_scores(leaf, t, top_k=3, ignore_index=0)
+    dx, = torch.autograd.grad([out.logp], [leaf], [torch.ones(rows, device="cuda")])
+    small = x.detach()[-3:].clone().requires_grad_()
+    ref = word_ops.token_scores(small, t[-3:], top_k=3, ignore_index=0)
+    dref, = torch.autograd.grad([ref.logp], [small], [torch.ones(3, device="cuda")])
+    assert torch.equal(out.top_ids[-3:], ref.top_ids) and bool((out.top_ids[:-3] == -1).all())
+    # another split of the rows over the waves may be taken for 3 rows than for 70000
+    assert bool(((out.logp[-3:] - ref.logp).abs() <= 2 * _log_tol(V, ref.logp)).all())
+    assert bool(((dx[-3:].float() - dref.float()).abs() <= 2.0 ** -8 * dref.float().abs() + 1e-6).all())
+    assert bool((dx[:-3:997] == 0).all())
+
+
+def test_more_rows_than_workgroups():
+    rows, V = (1 << 22) + 77, 3
+    x = _logits((rows,), V, torch.float32, 92)
+    t = _ints((rows,), V, 93)
+    leaf = x.requires_grad_()
+    out = word_ops.token_scores(leaf, t, top_k=1)
+    dx, = torch.autograd.grad([out.logp], [leaf], [torch.ones(rows, device="cuda")])
+    lq = torch.log_softmax(x.detach().double(), -1)
+    want = lq.gather(-1, t.unsqueeze(-1)).squeeze(-1)
+    assert bool(((out.logp.double() - want).abs() <= _log_tol(V, want)).all())
+    ref = torch.nn.functional.one_hot(t, V) - lq.exp()
+    assert float((dx.double() - ref).abs().max()) <= 400 * U
+    y = word_ops.embed_tokens(t, torch.eye(3, device="cuda"))
+    assert torch.equal(y.argmax(-1), t)
+
+
+def test_embed_table_past_32_bit_offsets():
+    V, D = 70000, 32768
+    table = torch.zeros(V, D, dtype=torch.bfloat16, device="cuda")
+    table[-1] = 1.0
+    leaf = table.requires_grad_()
+    t = torch.tensor([V - 1, 5, V - 1], device="cuda")
+    y = word_ops.embed_tokens(t, leaf, 3.0)
+    assert bool((y[0] == 3).all()) and bool((y[1] == 0).all())
+    d, = torch.autograd.grad([y], [leaf], [torch.ones_like(y)])
+    assert bool((d[-1] == 6).all()) and bool((d[5] == 3).all()) and bool((d[6:-1:501] == 0).all())
