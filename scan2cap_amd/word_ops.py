@@ -97,18 +97,38 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
-def _workspace(fn, argtypes, args, device):
-    f = getattr(_C.load(), fn)
-    f.argtypes, f.restype = argtypes, _LL
+_SIZES = {"s2c_token_scores_workspace_bytes": [_I] * 4, "s2c_distill_workspace_bytes": [_I] * 3,
+          "s2c_embed_grad_workspace_bytes": [_LL, _I, _I]}
+_size_fns = {}
+
+
+def _workspace(name, device, *args):
+    f = _size_fns.get(name)
+    if f is None:
+        f = getattr(_C.load(), name)
+        f.argtypes, f.restype = _SIZES[name], _LL
+        _size_fns[name] = f
     n = f(*args)
     return torch.empty(n, dtype=torch.uint8, device=device) if n else None
 
 
 def _run(name, device, *args, alg_bytes=0):
+    """One entry point on the device's current stream.  A training batch's launch takes 5 - 10 us, as long
+    as the Python around it: the device is switched only where it is another one, and the stream's handle
+    is asked for directly."""
     if _C.TIMER.enabled:
         _C.TIMER.alg_bytes = int(alg_bytes)
-    with torch.cuda.device(device):
-        _C.call(name, *args, _C.stream_ptr())
+    if device.index == torch._C._cuda_getDevice():
+        _C.call(name, *args, torch._C._cuda_getCurrentRawStream(device.index))
+    else:
+        with torch.cuda.device(device):
+            _C.call(name, *args, torch._C._cuda_getCurrentRawStream(device.index))
+
+
+def _f32(g):
+    if g is None or (g.dtype is torch.float32 and g.is_contiguous()):
+        return g
+    return g.to(torch.float32).contiguous()
 
 
 def _merge_axes(shape, strides):
@@ -128,16 +148,27 @@ def _logits(x, temperature):
     """x (..., V) as the kernels read it: (tensor, s2c_logits).  Up to three leading axes of any strides
     are read in place (a decoder's word-major logits permuted to (B, K, T, V)); more, or words that are
     not adjacent, are copied first."""
-    if x.shape[-1] > 1 and x.stride(-1) != 1:
+    V = x.shape[-1]
+    rows = x.numel() // V
+    if x.is_contiguous():
+        return x, _Logits(rows, V, _DTYPES[x.dtype], 1, max(rows, 1), 1.0 / temperature, 0, 0, V, x.data_ptr())
+    if V > 1 and x.stride(-1) != 1:
         x = x.contiguous()
     axes = _merge_axes(x.shape[:-1], x.stride()[:-1])
     if len(axes) > 3:
         x = x.contiguous()
         axes = _merge_axes(x.shape[:-1], x.stride()[:-1])
     axes = [(1, 0)] * (3 - len(axes)) + axes
-    rows = x.numel() // x.shape[-1]
-    return x, _Logits(rows, x.shape[-1], _DTYPES[x.dtype], axes[1][0], axes[2][0], 1.0 / temperature,
+    return x, _Logits(rows, V, _DTYPES[x.dtype], axes[1][0], axes[2][0], 1.0 / temperature,
                       axes[0][1], axes[1][1], axes[2][1], x.data_ptr())
+
+
+def _first_order(fn, ctx, grads):
+    """The gradients are not differentiable again; the guard that says so is put around them only where a
+    graph of the backward pass is asked for (create_graph)."""
+    if torch.is_grad_enabled():
+        return once_differentiable(fn._backward)(ctx, *grads)
+    return fn._backward(ctx, *grads)
 
 
 def _check_logits(x, temperature):
@@ -154,7 +185,7 @@ def _check_logits(x, temperature):
 class _TokenScores(Function):
     @staticmethod
     def forward(ctx, logits, tokens, top_k, temperature, ignore_index):
-        x, lg = _logits(logits.detach(), temperature)
+        x, lg = _logits(logits, temperature)
         shape, dev = logits.shape[:-1], logits.device
         f32 = dict(dtype=torch.float32, device=dev)
         logp = torch.empty(shape, **f32) if tokens is not None else None
@@ -163,37 +194,36 @@ class _TokenScores(Function):
         top_ids = torch.empty(shape + (top_k,), dtype=torch.int64, device=dev) if top_k else None
         stats = torch.empty((lg.rows, 4), **f32)
         args = _ScoresArgs(lg, top_k, int(ignore_index is not None), ignore_index or 0, _ptr(tokens),
-                           _ptr(logp), _ptr(entropy), _ptr(top_logp), _ptr(top_ids), _ptr(stats), None)
+                           _ptr(logp), entropy.data_ptr(), _ptr(top_logp), _ptr(top_ids), stats.data_ptr(),
+                           None)
         if lg.rows:
-            with torch.cuda.device(dev):
-                ws = _workspace("s2c_token_scores_workspace_bytes", [_I] * 4, (lg.rows, lg.V, lg.dtype, top_k),
-                                dev)
+            ws = _workspace("s2c_token_scores_workspace_bytes", dev, lg.rows, lg.V, lg.dtype, top_k)
             args.ws = _ptr(ws)
             _run("s2c_token_scores_fwd", dev, ctypes.addressof(args),
                  alg_bytes=x.numel() * x.element_size() + lg.rows * (16 + 12 * top_k))
-        ctx.save_for_backward(logits, tokens, top_ids, stats)
-        ctx.opts = (top_k, temperature, ignore_index)
+        ctx.set_materialize_grads(False)
         if top_ids is not None:
             ctx.mark_non_differentiable(top_ids)
-        ctx.set_materialize_grads(False)
+        if ctx.needs_input_grad[0]:
+            ctx.save_for_backward(x, tokens, top_ids, stats)      # what `args` points to
+            ctx.args, ctx.shape = args, logits.shape
         return logp, entropy, top_logp, top_ids
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, g_logp, g_entropy, g_top, _g_ids):
-        if g_logp is None and g_entropy is None and g_top is None:
-            return (None,) * 5
-        logits, tokens, top_ids, stats = ctx.saved_tensors
-        top_k, temperature, ignore_index = ctx.opts
-        x, lg = _logits(logits.detach(), temperature)
-        dx = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        if lg.rows:
-            g = [None if t is None else t.to(torch.float32).contiguous() for t in (g_logp, g_entropy, g_top)]
-            args = _ScoresArgs(lg, top_k, int(ignore_index is not None), ignore_index or 0, _ptr(tokens),
-                               None, None, None, _ptr(top_ids), _ptr(stats), None)
-            _run("s2c_token_scores_bwd", logits.device, ctypes.addressof(args), _ptr(g[0]), _ptr(g[1]),
-                 _ptr(g[2]), _ptr(dx), alg_bytes=2 * x.numel() * x.element_size())
+    def _backward(ctx, g_logp, g_entropy, g_top, _g_ids):
+        x = ctx.saved_tensors[0]
+        dx = torch.empty(ctx.shape, dtype=x.dtype, device=x.device)
+        if ctx.args.lg.rows:
+            if g_logp is None and g_entropy is None and g_top is None:
+                return None, None, None, None, None
+            gl, ge, gt = _f32(g_logp), _f32(g_entropy), _f32(g_top)
+            _run("s2c_token_scores_bwd", x.device, ctypes.addressof(ctx.args), _ptr(gl), _ptr(ge), _ptr(gt),
+                 dx.data_ptr(), alg_bytes=2 * x.numel() * x.element_size())
         return dx, None, None, None, None
+
+    @staticmethod
+    def backward(ctx, *grads):
+        return _first_order(_TokenScores, ctx, grads)
 
 
 def token_scores(logits, tokens=None, top_k=0, temperature=1.0, ignore_index=None):
@@ -228,37 +258,38 @@ def token_scores(logits, tokens=None, top_k=0, temperature=1.0, ignore_index=Non
 class _Distill(Function):
     @staticmethod
     def forward(ctx, logits, ids, teacher, mask, temperature):
-        x, lg = _logits(logits.detach(), temperature)
+        x, lg = _logits(logits, temperature)
         dev = logits.device
         loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=dev)
         stats = torch.empty((lg.rows, 4), dtype=torch.float32, device=dev)
+        args = _DistillArgs(lg, ids.shape[-1], _DTYPES[teacher.dtype], ids.data_ptr(), teacher.data_ptr(),
+                            _ptr(mask), loss.data_ptr(), stats.data_ptr(), None)
         if lg.rows:
-            with torch.cuda.device(dev):
-                ws = _workspace("s2c_distill_workspace_bytes", [_I] * 3, (lg.rows, lg.V, lg.dtype), dev)
-            args = _DistillArgs(lg, ids.shape[-1], _DTYPES[teacher.dtype], _ptr(ids), _ptr(teacher),
-                                _ptr(mask), _ptr(loss), _ptr(stats), _ptr(ws))
+            ws = _workspace("s2c_distill_workspace_bytes", dev, lg.rows, lg.V, lg.dtype)
+            args.ws = _ptr(ws)
             _run("s2c_distill_fwd", dev, ctypes.addressof(args),
                  alg_bytes=x.numel() * x.element_size() + ids.numel() * (8 + teacher.element_size()))
-        ctx.save_for_backward(logits, ids, teacher, stats)
-        ctx.temperature = temperature
         ctx.set_materialize_grads(False)
+        if ctx.needs_input_grad[0]:
+            ctx.save_for_backward(x, ids, teacher, stats)         # what `args` points to
+            ctx.args, ctx.shape = args, logits.shape
         return loss
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, g_loss):
+    def _backward(ctx, g_loss):
         if g_loss is None:
-            return (None,) * 5
-        logits, ids, teacher, stats = ctx.saved_tensors
-        x, lg = _logits(logits.detach(), ctx.temperature)
-        dx = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-        if lg.rows:
-            g = g_loss.to(torch.float32).contiguous()
-            args = _DistillArgs(lg, ids.shape[-1], _DTYPES[teacher.dtype], _ptr(ids), _ptr(teacher), None,
-                                None, _ptr(stats), None)
-            _run("s2c_distill_bwd", logits.device, ctypes.addressof(args), _ptr(g), _ptr(dx),
+            return None, None, None, None, None
+        x = ctx.saved_tensors[0]
+        dx = torch.empty(ctx.shape, dtype=x.dtype, device=x.device)
+        if ctx.args.lg.rows:
+            g = _f32(g_loss)
+            _run("s2c_distill_bwd", x.device, ctypes.addressof(ctx.args), g.data_ptr(), dx.data_ptr(),
                  alg_bytes=2 * x.numel() * x.element_size())
         return dx, None, None, None, None
+
+    @staticmethod
+    def backward(ctx, *grads):
+        return _first_order(_Distill, ctx, grads)
 
 
 def distill_loss(logits, teacher_ids, teacher_logits, temperature=1.0, mask=None):
@@ -297,35 +328,41 @@ class _EmbedTokens(Function):
     @staticmethod
     def forward(ctx, tokens, table, scale, padding):
         (V, D), N, dev = table.shape, tokens.numel(), table.device
-        out = torch.empty(tuple(tokens.shape) + (D,), dtype=table.dtype, device=dev)
+        out = torch.empty(tokens.shape + (D,), dtype=table.dtype, device=dev)
         if N and D:
-            _run("s2c_embed_fwd", dev, N, V, D, _DTYPES[table.dtype], table.stride(0), _ptr(tokens),
-                 _ptr(table), scale, padding, _ptr(out), alg_bytes=2 * out.numel() * out.element_size())
-        ctx.save_for_backward(tokens)
-        ctx.opts = (V, D, table.dtype, scale, padding)
+            _run("s2c_embed_fwd", dev, N, V, D, _DTYPES[table.dtype], table.stride(0), tokens.data_ptr(),
+                 table.data_ptr(), scale, padding, out.data_ptr(),
+                 alg_bytes=2 * out.numel() * out.element_size())
         ctx.set_materialize_grads(False)
+        if ctx.needs_input_grad[1]:
+            ctx.save_for_backward(tokens)
+            ctx.opts = (N, V, D, table.dtype, scale, padding)
         return out
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, g):
+    def _backward(ctx, g):
         if g is None:
-            return (None,) * 4
+            return None, None, None, None
         tokens, = ctx.saved_tensors
-        V, D, dtype, scale, padding = ctx.opts
-        N = tokens.numel()
-        d_table = torch.empty((V, D), dtype=dtype, device=g.device)
+        N, V, D, dtype, scale, padding = ctx.opts
+        dev = g.device
+        d_table = torch.empty((V, D), dtype=dtype, device=dev)
         if D:
-            axes = _merge_axes(g.shape[:-1], g.stride()[:-1])
-            if len(axes) > 1 or (D > 1 and g.stride(-1) != 1):
-                g = g.contiguous()
-                axes = [(N, D)]
-            with torch.cuda.device(g.device):
-                ws = _workspace("s2c_embed_grad_workspace_bytes", [_LL, _I, _I], (N, V, D), g.device)
-            _run("s2c_embed_grad", g.device, N, V, D, _DTYPES[dtype], axes[0][1] if axes else D,
-                 _ptr(tokens) if N else None, _ptr(g) if N else None, scale, padding, _ptr(d_table), _ptr(ws),
-                 alg_bytes=(N * D + V * D) * g.element_size())
+            ld = D
+            if not g.is_contiguous():
+                axes = _merge_axes(g.shape[:-1], g.stride()[:-1])
+                if len(axes) > 1 or (D > 1 and g.stride(-1) != 1):
+                    g = g.contiguous()
+                elif axes:
+                    ld = axes[0][1]
+            ws = _workspace("s2c_embed_grad_workspace_bytes", dev, N, V, D)
+            _run("s2c_embed_grad", dev, N, V, D, _DTYPES[dtype], ld, tokens.data_ptr(), g.data_ptr(), scale,
+                 padding, d_table.data_ptr(), _ptr(ws), alg_bytes=(N * D + V * D) * g.element_size())
         return None, d_table, None, None
+
+    @staticmethod
+    def backward(ctx, *grads):
+        return _first_order(_EmbedTokens, ctx, grads)
 
 
 def embed_tokens(tokens, table, scale=1.0, padding_idx=None):

@@ -536,6 +536,19 @@ def test_operators_together():
     assert float((dW.double() - wW).abs().max()) <= 1e-5 * float(wW.abs().max())
 
 
+def test_second_derivatives_are_refused():
+    x = _logits((3,), 50, torch.float32, 62).requires_grad_()
+    table = _logits((50,), 4, torch.float32, 63).requires_grad_()
+    t, ids = _ints((3,), 50, 64), _ints((3, 2), 50, 65)
+    for leaf, y in ((x, word_ops.token_scores(x, t).logp), (table, word_ops.embed_tokens(t, table)),
+                    (x, word_ops.distill_loss(x, ids, torch.zeros(3, 2, device="cuda")))):
+        w = torch.ones_like(y).requires_grad_()
+        g, = torch.autograd.grad([y], [leaf], [w], create_graph=True)
+        assert bool(g.isfinite().all())
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            g.sum().backward()
+
+
 def test_on_another_stream():
     ins = _pipeline_inputs(61)
     want = _pipeline(*ins)
