@@ -11,18 +11,20 @@
 // NaN and +inf reach s0 and with it every output of the row.
 //
 // The k best: keys (order-preserving 32 bits of the value | ~index) make equal values unique, lowest
-// index first.  A wave keeps candidates in LDS and a threshold tau: the k-th best value it is sure of.
-// The first tile takes tau from the 64 lanes' tile maxima (k-th largest of them, a binary search over
-// ballots), later tiles are entered only if some lane's tile maximum is above tau, and the buffer is cut
-// back to its k best, by counting ranks, when it fills.  Later elements equal to tau lose their tie: a
-// wave walks its tiles in index order.
+// index first.  A wave keeps candidates in LDS and enters a tile only where some lane's tile maximum
+// passes a threshold, a lower bound of the row's k-th best value.  The first bound is the k-th largest of
+// 64 maxima (a binary search over ballots), each over one lane's elements in the first tiles of all waves
+// of the group; an element equal to it may still win by its index.  When the buffer fills it is cut back
+// to its k best, by counting ranks; later elements equal to a wave's own k-th have lost, since a wave
+// walks its tiles in index order.
 //
 // All of it is bound by reading the logits (and, backward, reading them again and writing the
 // gradient).
 #include "s2c_words_common.h"
 
-#include <limits.h>
 #include <stdio.h>
+
+#include <type_traits>
 
 using namespace s2c;
 
@@ -33,8 +35,8 @@ constexpr float LN2 = 0.69314718055994530942f;
 constexpr int KMAX = S2C_WORDS_MAX_TOP;
 constexpr int SLOTS = S2C_WORDS_MAX_SLOTS;
 constexpr int BUF = 192;          // candidates of a wave: cut back when more than BUF - 64 are held
-constexpr int THREADS = 256, WAVES = THREADS / 64;
 constexpr int U = 4;              // 16-byte loads in flight per lane
+constexpr int MAX_SPLIT = 64;     // stretches of a row (the lanes that join them)
 
 __device__ __forceinline__ float exp2_(float v) { return __builtin_amdgcn_exp2f(v); }
 __device__ __forceinline__ float nan_max(float a, float b) { return __builtin_elementwise_maximum(a, b); }
@@ -62,11 +64,11 @@ __device__ __forceinline__ float from(u32 k) {
   if (t == 0x7FFFFFFFu) --t;
   return unord(t);
 }
-// a lower bound of the k-th largest of the 64 lanes' keys, its upper 20 bits (0: fewer than k keys)
+// a lower bound of the k-th largest of the 64 lanes' keys, its upper 16 bits (0: fewer than k keys)
 __device__ __forceinline__ u32 kth_of_lanes(u32 key, int k) {
   u32 cur = 0;
 #pragma unroll
-  for (int b = 31; b >= 12; --b) {
+  for (int b = 31; b >= 16; --b) {
     const u32 trial = cur | (1u << b);
     if (__popcll(__ballot(key >= trial)) >= k) cur = trial;
   }
@@ -77,22 +79,31 @@ __device__ __forceinline__ u32 kth_of_lanes(u32 key, int k) {
 struct Best {
   u64 *buf;
   int cnt, k;
-  u32 tau;           // keys above tau are wanted
-  u64 kth;           // the k-th best key held after the last cut, 0 if fewer are held
+  u32 bound;         // keys below it are not wanted
+  u64 kth;           // the k-th best key held at the last cut, 0 if fewer were held
 
-  __device__ __forceinline__ void init(u64 *b, int k_) { buf = b; k = k_; cnt = 0; tau = 0; kth = 0; }
+  __device__ __forceinline__ void init(u64 *b, int k_) { buf = b; k = k_; cnt = 0; bound = 0; kth = 0; }
+  // values that pass: !(x <= threshold)
+  __device__ __forceinline__ float threshold() const {
+    const u32 t = (u32)(kth >> 32);
+    return kth && t >= bound ? above(t) : from(bound);
+  }
 
-  // keep the k best, in descending order
+  // keep the k best, in descending order: an entry's rank is the number of greater ones
   __device__ __forceinline__ void cut(int lane) {
     wave_lds_fence();
     u64 e[3];
     int rank[3] = {0, 0, 0};
 #pragma unroll
     for (int i = 0; i < 3; ++i) e[i] = lane + 64 * i < cnt ? buf[lane + 64 * i] : 0;
-    for (int j = 0; j < cnt; ++j) {
-      const u64 o = buf[j];
+    if (cnt <= 64) {            // the common case stays in registers
+      for (int j = 0; j < cnt; ++j) rank[0] += readlane_u64(e[0], j) > e[0];
+    } else {
+      for (int j = 0; j < cnt; ++j) {
+        const u64 o = buf[j];
 #pragma unroll
-      for (int i = 0; i < 3; ++i) rank[i] += o > e[i];
+        for (int i = 0; i < 3; ++i) rank[i] += o > e[i];
+      }
     }
     wave_lds_fence();
 #pragma unroll
@@ -102,17 +113,16 @@ struct Best {
     if (cnt >= k) {
       cnt = k;
       kth = buf[k - 1];
-      const u32 t = (u32)(kth >> 32);
-      if (t > tau) tau = t;
     }
   }
-  // lanes with `f` add `key`; true if the buffer was cut for it
-  __device__ __forceinline__ bool add(u64 mask, u64 key, int lane) {
-    bool was_cut = false;
-    if (cnt > BUF - 64) { cut(lane); was_cut = true; }
+  // the lanes of `mask` add `key`
+  __device__ __forceinline__ void add(u64 mask, u64 key, int lane) {
+    if (cnt > BUF - 64) {
+      cut(lane);
+      mask &= __ballot(key > kth);
+    }
     if ((mask >> lane) & 1) buf[cnt + mask_rank_below(mask)] = key;
     cnt += __popcll(mask);
-    return was_cut;
   }
 };
 
@@ -123,16 +133,19 @@ __device__ __forceinline__ void merge_lists(Best &b, int L, int lane, F key) {
   const int ppl = 64 / L;
   const int list = lane & (L - 1), sub = lane / L;
   u64 thr = 0;
+  u64 next = sub < b.k ? key(list, sub) : 0;
   for (int p0 = 0; p0 < b.k; p0 += ppl) {
-    const int pos = p0 + sub;
-    const u64 v = pos < b.k ? key(list, pos) : 0;
+    const u64 v = next;
+    const int ahead = p0 + ppl + sub;
+    next = ahead < b.k ? key(list, ahead) : 0;
     if (p0 == 0) {
-      const u32 cur = kth_of_lanes((u32)(v >> 32), b.k);
-      thr = cur ? ((u64)cur << 32) - 1 : 0;
+      const u32 bound = kth_of_lanes((u32)(v >> 32), b.k);
+      thr = bound ? ((u64)bound << 32) - 1 : 0;
     }
     const u64 mask = __ballot(v > thr);
     if (mask == 0) break;
-    if (b.add(mask, v, lane) && b.kth) thr = b.kth;
+    b.add(mask, v, lane);
+    if (b.kth > thr) thr = b.kth;
   }
   b.cut(lane);
 }
@@ -153,101 +166,118 @@ __device__ __forceinline__ Stat wave_combine(Stat s, float c) {
   return o;
 }
 
-// one wave's share of a row: tiles of 64 U vectors, wave `w` of `nw`, vectors [vb, ve) of the row
-template <int DT, bool TOP, bool ENT>
-__device__ __forceinline__ Stat stream_row(const char *xr, int V, int vb, int ve, int w, int nw, float c,
-                                           Best &best) {
+// One tile of a row: 64 U vectors from vector t0.  INSIDE: all of it lies in the row and the stretch [.., ve),
+// its loads carry no condition and are under way together; else `nu` of its U vectors a lane may.
+template <int DT, int G, bool TOP, bool ENT, bool INSIDE>
+__device__ __forceinline__ void stream_tile(const char *xr, int V, int shift, int t0, int ve, float c, bool first,
+                                            Stat &s, Best &best, u32 *s_max) {
   typedef Elem<DT> E;
   constexpr int VEC = E::VEC;
   const int lane = lane_id();
-  const int shift = (int)(((uintptr_t)xr / E::ES) & (VEC - 1));   // vector i = elements i VEC - shift ..
-  Stat s = {-INFINITY, 0.0f, 0.0f};
-  bool first = true;
-  for (int t0 = vb + w * 64 * U; t0 < ve; t0 += nw * 64 * U) {
-    Raw r[U];
-    if ((long long)t0 * VEC - shift >= 0 && (long long)(t0 + 64 * U) * VEC - shift <= V && t0 + 64 * U <= ve) {
+  const int nu = INSIDE ? U : t0 < ve ? min(U, (ve - t0 + 63) >> 6) : 0;
+  Raw r[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        r[u] = *reinterpret_cast<const Raw *>(xr + ((long long)(t0 + u * 64 + lane) * VEC - shift) * E::ES);
+  for (int u = 0; u < U; ++u) {
+    const int vi = t0 + u * 64 + lane;
+    const long long e0 = (long long)vi * VEC - shift;
+    if (INSIDE) {
+      r[u] = *reinterpret_cast<const Raw *>(xr + e0 * E::ES);
     } else {
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int vi = t0 + u * 64 + lane;
-        const long long e0 = (long long)vi * VEC - shift;
+      for (int i = 0; i < 4; ++i) r[u].w[i] = E::NEG_INF;
+      if (vi < ve) {
+        if (e0 >= 0 && e0 + VEC <= V) {
+          r[u] = *reinterpret_cast<const Raw *>(xr + e0 * E::ES);
+        } else {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) r[u].w[i] = E::NEG_INF;
-        if (vi < ve) {
-          if (e0 >= 0 && e0 + VEC <= V) {
-            r[u] = *reinterpret_cast<const Raw *>(xr + e0 * E::ES);
-          } else {
-#pragma unroll
-            for (int e = 0; e < VEC; ++e)
-              if (e0 + e >= 0 && e0 + e < V) E::put(r[u], e, E::bits(xr, e0 + e));
-          }
+          for (int e = 0; e < VEC; ++e)
+            if (e0 + e >= 0 && e0 + e < V) E::put(r[u], e, E::bits(xr, e0 + e));
         }
       }
-    }
-    float tmax = E::at(r[0], 0);
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) tmax = nan_max(tmax, E::at(r[u], e));
-
-    if (TOP) {
-      bool enter = true;
-      float thr;
-      u32 next = best.tau;
-      if (first) {
-        const long long e0 = (long long)(t0 + lane) * VEC - shift;     // the lane's lowest element
-        const bool any = t0 + lane < ve && e0 < V;
-        next = kth_of_lanes(any ? ord(tmax) : 0u, best.k);
-        thr = from(next);
-      } else {
-        thr = above(best.tau);
-        enter = __ballot(!(tmax <= thr)) != 0;
-      }
-      if (enter) {
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-#pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            const float v = E::at(r[u], e);
-            u64 mask = __ballot(!(v <= thr));
-            if (mask) {
-              const int vi = t0 + u * 64 + lane;
-              const long long idx = (long long)vi * VEC - shift + e;
-              mask &= __ballot(vi < ve && idx >= 0 && idx < V);
-              const u64 key = ((u64)ord(v) << 32) | (u32)~(u32)idx;
-              // after a cut inside a tile, elements equal to the new tau may still win by their index
-              if (mask && best.add(mask, key, lane)) thr = from(best.tau > next ? best.tau : next);
-            }
-          }
-        }
-      }
-      if (next > best.tau) best.tau = next;
-      first = false;
-    }
-
-    const float m_new = nan_max(s.m, tmax);
-    const float delta = fmaxf((s.m - m_new) * c, D_MIN), a = exp2_(delta);
-    const float mref = finite_or_0(m_new);
-    s.s1 = a * (s.s1 + delta * s.s0);
-    s.s0 = a * s.s0;
-    s.m = m_new;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float p0 = 0.0f, p1 = 0.0f;
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const float d = (E::at(r[u], e) - mref) * c;
-        const float ex = exp2_(d);
-        p0 += ex;
-        if (ENT) p1 = __builtin_fmaf(ex, fmaxf(d, D_MIN), p1);
-      }
-      s.s0 += p0;
-      if (ENT) s.s1 += p1;
     }
   }
+  float tmax = -INFINITY;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (!INSIDE && u >= nu) break;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) tmax = nan_max(tmax, E::at(r[u], e));
+  }
+
+  if (TOP) {
+    if (first) {
+      const long long e0 = (long long)(t0 + lane) * VEC - shift;     // the lane's lowest element
+      u32 key = t0 + lane < ve && e0 < V ? ord(tmax) : 0u;
+      if (G > 1) {
+        atomicMax(&s_max[lane], key);
+        __syncthreads();
+        key = s_max[lane];
+      }
+      best.bound = kth_of_lanes(key, best.k);
+    }
+    const float thr = best.threshold();
+    if (__ballot(!(tmax <= thr))) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (!INSIDE && u >= nu) break;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const float v = E::at(r[u], e);
+          u64 mask = __ballot(!(v <= thr));
+          if (mask) {
+            const int vi = t0 + u * 64 + lane;
+            const u32 idx = (u32)vi * VEC - shift + e;               // (negative: above V)
+            const u64 key = ((u64)ord(v) << 32) | (u32)~idx;
+            if (!INSIDE) mask &= __ballot(vi < ve && idx < (u32)V);
+            if (best.kth) mask &= __ballot(key > best.kth);
+            if (mask) best.add(mask, key, lane);
+          }
+        }
+      }
+    }
+  }
+
+  const float m_new = nan_max(s.m, tmax);
+  const float delta = fmaxf((s.m - m_new) * c, D_MIN), a = exp2_(delta);
+  const float mref = finite_or_0(m_new);
+  s.s1 = a * (s.s1 + delta * s.s0);
+  s.s0 = a * s.s0;
+  s.m = m_new;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (!INSIDE && u >= nu) break;
+    float p0 = 0.0f, p1 = 0.0f;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) {
+      const float d = (E::at(r[u], e) - mref) * c;
+      const float ex = exp2_(d);
+      p0 += ex;
+      if (ENT) p1 = __builtin_fmaf(ex, fmaxf(d, D_MIN), p1);
+    }
+    s.s0 += p0;
+    if (ENT) s.s1 += p1;
+  }
+}
+
+// one wave's share of a row: wave `w` of the `G` of a group, vectors [vb, ve) of the row.  s_max (64, zero):
+// the group's lane maxima.
+template <int DT, int G, bool TOP, bool ENT>
+__device__ __forceinline__ Stat stream_row(const char *xr, int V, int vb, int ve, int w, float c, Best &best,
+                                           u32 *s_max) {
+  constexpr int VEC = Elem<DT>::VEC;
+  const int shift = (int)(((uintptr_t)xr / Elem<DT>::ES) & (VEC - 1));   // vector i = elements i VEC - shift ..
+  const int full = (int)(((long long)V + shift) / VEC);                    // whole vectors end here
+  const int last = min(ve, full), begin = vb + w * 64 * U;
+  Stat s = {-INFINITY, 0.0f, 0.0f};
+  int t0 = begin;
+  if (!(TOP && G > 1) && t0 >= ve) return s;                               // (else every wave gives its maxima)
+  do {
+    if ((t0 > 0 || shift == 0) && t0 + 64 * U <= last)
+      stream_tile<DT, G, TOP, ENT, true>(xr, V, shift, t0, ve, c, t0 == begin, s, best, s_max);
+    else
+      stream_tile<DT, G, TOP, ENT, false>(xr, V, shift, t0, ve, c, t0 == begin, s, best, s_max);
+    t0 += G * 64 * U;
+  } while (t0 < ve);
   return wave_combine(s, c);
 }
 
@@ -255,6 +285,78 @@ __device__ __forceinline__ Stat stream_row(const char *xr, int V, int vb, int ve
 // stats: {mref, log2 s0, ., .}; log2 s0 = +inf marks a row without gradient, NaN one whose gradient is NaN
 __device__ __forceinline__ float log2_sum(const Stat &s) {
   return s.s0 == 0.0f ? INFINITY : log2f(s.s0);        // (0: every logit is -inf)
+}
+
+// G waves of a workgroup share a row's stretch: waves per workgroup, groups per workgroup
+template <int G> struct Shape {
+  static constexpr int WAVES = G == 1 ? 4 : G, THREADS = 64 * WAVES, GROUPS = WAVES / G;
+};
+
+// the partial results of a row that several workgroups read
+struct Split {
+  int n;               // stretches per row, a power of two; 1: none
+  Stat *part;          // (rows, n)
+  u64 *keys;           // (rows, n, k)
+};
+
+// Statistics (and, TOP, the k best) of stretch `seg` of `segs` of a row, by the G waves of a group.
+// Wave 0 of the group gets the result; its k best are in `lists[G > 1 ? G : 0]`, 0 after the last one.
+// Every wave of the workgroup comes here together where G > 1.
+template <int DT, int G, bool TOP, bool ENT>
+__device__ __forceinline__ Stat group_stat(const char *xr, int V, int seg, int segs, int k, float c,
+                                           u64 (*lists)[BUF], Stat *s_part, u32 *s_max) {
+  typedef Elem<DT> E;
+  const int lane = lane_id(), w = G == 1 ? 0 : (int)(threadIdx.x >> 6);
+  const int shift = (int)(((uintptr_t)xr / E::ES) & (E::VEC - 1));
+  const int nvec = (int)(((long long)V + shift + E::VEC - 1) / E::VEC);
+  const int per = (nvec + segs - 1) / segs;
+  const int vb = min(nvec, seg * per), ve = min(nvec, vb + per);
+  Best best;
+  if (TOP) best.init(lists[w], k);
+  Stat s = stream_row<DT, G, TOP, ENT>(xr, V, vb, ve, w, c, best, s_max);
+  if (TOP) {
+    best.cut(lane);
+    for (int j = best.cnt + lane; j < k; j += 64) lists[w][j] = 0;
+    wave_lds_fence();
+  }
+  if (G > 1) {
+    if (lane == 0) s_part[w] = s;
+    __syncthreads();
+    if (w == 0) {
+      Stat o = {-INFINITY, 0.0f, 0.0f};
+      if (lane < G) o = s_part[lane];
+      s = wave_combine(o, c);
+      if (TOP) {
+        s_max[lane] = 0;                     // (read by all, needed again after the workgroup's next barrier)
+        Best all;
+        all.init(lists[G], k);
+        merge_lists(all, G, lane, [&](int list, int pos) { return lists[list][pos]; });
+        for (int j = all.cnt + lane; j < k; j += 64) lists[G][j] = 0;
+        wave_lds_fence();
+      }
+    }
+  }
+  return s;
+}
+
+// a wave joins the stretches of a row; the k best go to `list`
+__device__ __forceinline__ Stat join_stretches(const Split &sp, int r, int k, float c, u64 *list, int lane) {
+  Stat o = {-INFINITY, 0.0f, 0.0f};
+  if (lane < sp.n) o = sp.part[(size_t)r * sp.n + lane];
+  o = wave_combine(o, c);
+  if (k) {
+    Best all;
+    all.init(list, k);
+    const u64 *keys = sp.keys + (size_t)r * sp.n * k;
+    merge_lists(all, sp.n, lane, [&](int l, int pos) { return keys[(size_t)l * k + pos]; });
+  }
+  return o;
+}
+
+__device__ __forceinline__ void write_part(const Split &sp, size_t unit, const Stat &s, const u64 *list, int k,
+                                           int lane) {
+  if (lane == 0) sp.part[unit] = s;
+  if (lane < k) sp.keys[unit * k + lane] = list[lane];
 }
 
 __device__ __forceinline__ bool scores_dead(const s2c_token_scores_args &a, int r) {
@@ -299,44 +401,51 @@ __device__ __forceinline__ void scores_write(const s2c_token_scores_args &a, int
   }
 }
 
-template <int DT>
-__global__ __launch_bounds__(THREADS) void scores_fwd_kernel(s2c_token_scores_args a) {
-  __shared__ u64 s_buf[WAVES + 1][BUF];
-  __shared__ Stat s_part[WAVES];
+template <int DT, int G, bool TOP>
+__global__ __launch_bounds__(Shape<G>::THREADS) void scores_fwd_kernel(s2c_token_scores_args a, Split sp) {
+  typedef Shape<G> Sh;
+  __shared__ u64 s_lists[TOP ? Sh::WAVES + (G > 1) : 1][TOP ? BUF : 1];
+  __shared__ Stat s_part[Sh::WAVES];
+  __shared__ u32 s_max[64];
   const int lane = lane_id(), w = threadIdx.x >> 6;
+  const int grp = G == 1 ? w : 0;
+  const bool first = G == 1 || w == 0;
+  if (TOP && G > 1) {
+    if (w == 0) s_max[lane] = 0;
+    __syncthreads();
+  }
+  u64 (*lists)[BUF] = reinterpret_cast<u64 (*)[BUF]>(&s_lists[TOP ? grp : 0][0]);
   const float c = a.lg.inv_t * LOG2E;
-  for (int r = blockIdx.x; r < a.lg.rows; r += gridDim.x) {
+  const long long units = (long long)a.lg.rows * sp.n;
+  for (long long un = (long long)blockIdx.x * Sh::GROUPS + grp; un < units; un += (long long)gridDim.x * Sh::GROUPS) {
+    const int r = (int)(un / sp.n), seg = (int)(un % sp.n);
     if (scores_dead(a, r)) {
-      if (w == 0) scores_write_dead(a, r, lane);
+      if (first && sp.n == 1) scores_write_dead(a, r, lane);
       continue;
     }
     const char *xr = row_ptr(a.lg, Elem<DT>::ES, r);
-    const int shift = (int)(((uintptr_t)xr / Elem<DT>::ES) & (Elem<DT>::VEC - 1));
-    const int nvec = (int)(((long long)a.lg.V + shift + Elem<DT>::VEC - 1) / Elem<DT>::VEC);
-    Best best;
-    best.init(s_buf[w], a.k);
-    Stat s;
-    if (a.k) {
-      s = stream_row<DT, true, true>(xr, a.lg.V, 0, nvec, w, WAVES, c, best);
-      best.cut(lane);
-      for (int j = best.cnt + lane; j < a.k; j += 64) s_buf[w][j] = 0;
-    } else {
-      s = stream_row<DT, false, true>(xr, a.lg.V, 0, nvec, w, WAVES, c, best);
+    const Stat s = group_stat<DT, G, TOP, true>(xr, a.lg.V, seg, sp.n, a.k, c, lists, s_part, s_max);
+    if (first) {
+      const u64 *list = lists[G > 1 ? G : 0];
+      if (sp.n == 1) scores_write<DT>(a, r, xr, s, list, lane);
+      else write_part(sp, (size_t)un, s, list, a.k, lane);
     }
-    if (lane == 0) s_part[w] = s;
-    __syncthreads();
-    if (w == 0) {
-      Stat o = {-INFINITY, 0.0f, 0.0f};
-      if (lane < WAVES) o = s_part[lane];
-      o = wave_combine(o, c);
-      if (a.k) {
-        Best all;
-        all.init(s_buf[WAVES], a.k);
-        merge_lists(all, WAVES, lane, [&](int list, int pos) { return s_buf[list][pos]; });
-      }
-      scores_write<DT>(a, r, xr, o, s_buf[WAVES], lane);
+    if (G > 1) __syncthreads();
+  }
+}
+
+template <int DT>
+__global__ __launch_bounds__(256) void scores_join_kernel(s2c_token_scores_args a, Split sp) {
+  __shared__ u64 s_list[4][BUF];
+  const int lane = lane_id(), w = threadIdx.x >> 6;
+  const float c = a.lg.inv_t * LOG2E;
+  for (long long r = (long long)blockIdx.x * 4 + w; r < a.lg.rows; r += (long long)gridDim.x * 4) {
+    if (scores_dead(a, (int)r)) {
+      scores_write_dead(a, (int)r, lane);
+      continue;
     }
-    __syncthreads();
+    const Stat s = join_stretches(sp, (int)r, a.k, c, s_list[w], lane);
+    scores_write<DT>(a, (int)r, row_ptr(a.lg, Elem<DT>::ES, (int)r), s, s_list[w], lane);
   }
 }
 
@@ -384,8 +493,15 @@ __device__ __forceinline__ void distill_write_dead(const s2c_distill_args &a, in
   }
 }
 
+// the student's logits at a lane's slots (asked for before the row is read)
 template <int DT>
-__device__ __forceinline__ void distill_write(const s2c_distill_args &a, int r, const char *xr,
+__device__ __forceinline__ void gather_slots(float (&at)[SLOTS / 64], const char *xr, int V, const Slots &t) {
+#pragma unroll
+  for (int i = 0; i < SLOTS / 64; ++i)
+    at[i] = t.id[i] >= 0 && t.id[i] < V ? Elem<DT>::load(xr, t.id[i]) : 0.0f;
+}
+
+__device__ __forceinline__ void distill_write(const s2c_distill_args &a, int r, const float (&at)[SLOTS / 64],
                                               const Stat &s, const Slots &t, int lane) {
   const float mref = finite_or_0(s.m);
   const float l2s = log2_sum(s);
@@ -396,7 +512,7 @@ __device__ __forceinline__ void distill_write(const s2c_distill_args &a, int r, 
   for (int i = 0; i < SLOTS / 64; ++i) {
     if (t.q[i] != 0.0f) {                       // (empty slots and vanishing ones add nothing; NaN does)
       if (t.id[i] >= a.lg.V) bad = true;
-      else part += t.q[i] * (t.lq[i] - ((Elem<DT>::load(xr, t.id[i]) - mref) * a.lg.inv_t - LN2 * sub));
+      else part += t.q[i] * (t.lq[i] - ((at[i] - mref) * a.lg.inv_t - LN2 * sub));
     }
   }
   part = wave_sum(part);
@@ -407,35 +523,57 @@ __device__ __forceinline__ void distill_write(const s2c_distill_args &a, int r, 
   }
 }
 
+template <int DT, int G>
+__global__ __launch_bounds__(Shape<G>::THREADS) void distill_fwd_kernel(s2c_distill_args a, Split sp) {
+  typedef Shape<G> Sh;
+  __shared__ Stat s_part[Sh::WAVES];
+  const int lane = lane_id(), w = threadIdx.x >> 6;
+  const int grp = G == 1 ? w : 0;
+  const bool first = G == 1 || w == 0;
+  const float c = a.lg.inv_t * LOG2E;
+  const long long units = (long long)a.lg.rows * sp.n;
+  for (long long un = (long long)blockIdx.x * Sh::GROUPS + grp; un < units; un += (long long)gridDim.x * Sh::GROUPS) {
+    const int r = (int)(un / sp.n), seg = (int)(un % sp.n);
+    bool dead = a.mask && a.mask[r] == 0;
+    const char *xr = row_ptr(a.lg, Elem<DT>::ES, r);
+    Slots t;
+    float at[SLOTS / 64];
+    if (!dead && sp.n == 1) {
+      t = load_slots(a, r, c, lane);
+      dead = t.l2w == INFINITY;
+      if (!dead) gather_slots<DT>(at, xr, a.lg.V, t);
+    }
+    if (dead) {
+      if (first && sp.n == 1) distill_write_dead(a, r, lane);
+      continue;
+    }
+    const Stat s = group_stat<DT, G, false, false>(xr, a.lg.V, seg, sp.n, 0, c, nullptr, s_part, nullptr);
+    if (first) {
+      if (sp.n == 1) distill_write(a, r, at, s, t, lane);
+      else write_part(sp, (size_t)un, s, nullptr, 0, lane);
+    }
+    if (G > 1) __syncthreads();
+  }
+}
+
 template <int DT>
-__global__ __launch_bounds__(THREADS) void distill_fwd_kernel(s2c_distill_args a) {
-  __shared__ Stat s_part[WAVES];
+__global__ __launch_bounds__(256) void distill_join_kernel(s2c_distill_args a, Split sp) {
   const int lane = lane_id(), w = threadIdx.x >> 6;
   const float c = a.lg.inv_t * LOG2E;
-  for (int r = blockIdx.x; r < a.lg.rows; r += gridDim.x) {
+  for (long long r = (long long)blockIdx.x * 4 + w; r < a.lg.rows; r += (long long)gridDim.x * 4) {
     bool dead = a.mask && a.mask[r] == 0;
     Slots t;
     if (!dead) {
-      t = load_slots(a, r, c, lane);
+      t = load_slots(a, (int)r, c, lane);
       dead = t.l2w == INFINITY;
     }
     if (dead) {
-      if (w == 0) distill_write_dead(a, r, lane);
+      distill_write_dead(a, (int)r, lane);
       continue;
     }
-    const char *xr = row_ptr(a.lg, Elem<DT>::ES, r);
-    const int shift = (int)(((uintptr_t)xr / Elem<DT>::ES) & (Elem<DT>::VEC - 1));
-    const int nvec = (int)(((long long)a.lg.V + shift + Elem<DT>::VEC - 1) / Elem<DT>::VEC);
-    Best none;
-    const Stat s = stream_row<DT, false, false>(xr, a.lg.V, 0, nvec, w, WAVES, c, none);
-    if (lane == 0) s_part[w] = s;
-    __syncthreads();
-    if (w == 0) {
-      Stat o = {-INFINITY, 0.0f, 0.0f};
-      if (lane < WAVES) o = s_part[lane];
-      distill_write<DT>(a, r, xr, wave_combine(o, c), t, lane);
-    }
-    __syncthreads();
+    float at[SLOTS / 64];
+    gather_slots<DT>(at, row_ptr(a.lg, Elem<DT>::ES, (int)r), a.lg.V, t);
+    distill_write(a, (int)r, at, join_stretches(sp, (int)r, 0, c, nullptr, lane), t, lane);
   }
 }
 
@@ -444,75 +582,15 @@ __global__ __launch_bounds__(THREADS) void distill_fwd_kernel(s2c_distill_args a
 //   scores  A = -(g + sum g_top + g_H H) inv_t, B = -g_H ln 2 inv_t, entries g inv_t at the token and
 //           g_top_j inv_t at top_ids_j
 //   distill A = g inv_t, B = 0, entries -g q_j inv_t at id_j
-// A workgroup writes the dense part of a stretch of a row, then the first entry of every word in the
-// stretch recomputes that element with all entries of the same word added, in slot order, and stores it
-// again (rounded once; no atomics).
-template <int DT>
-__device__ __forceinline__ void dense_row(const char *xr, void *dx, long long o0, int V, int vb, int ve,
-                                          int shift, float mref, float l2s, float A, float B, float c) {
-  typedef Elem<DT> E;
-  constexpr int VEC = E::VEC;
-  auto grad = [&](float x) {
-    const float d = (x - mref) * c - l2s;
-    return exp2_(d) * __builtin_fmaf(B, fmaxf(d, D_MIN), A);
-  };
-  for (int vi = vb + (int)threadIdx.x; vi < ve; vi += THREADS) {
-    const long long e0 = (long long)vi * VEC - shift;
-    if (e0 >= 0 && e0 + VEC <= V) {
-      const Raw r = load16<DT>(xr, e0);
-      float f[VEC];
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) f[e] = grad(E::at(r, e));
-      store16<DT>(dx, o0 + e0, E::pack(f));
-    } else {
-      for (int e = 0; e < VEC; ++e)
-        if (e0 + e >= 0 && e0 + e < V) E::store(dx, o0 + e0 + e, grad(E::load(xr, e0 + e)));
-    }
-  }
-}
-
-template <int DT>
-__device__ __forceinline__ void zero_row(void *dx, long long o0, int V, int vb, int ve, int shift) {
-  typedef Elem<DT> E;
-  constexpr int VEC = E::VEC;
-  const Raw z = {{0u, 0u, 0u, 0u}};
-  for (int vi = vb + (int)threadIdx.x; vi < ve; vi += THREADS) {
-    const long long e0 = (long long)vi * VEC - shift;
-    if (e0 >= 0 && e0 + VEC <= V) {
-      store16<DT>(dx, o0 + e0, z);
-    } else {
-      for (int e = 0; e < VEC; ++e)
-        if (e0 + e >= 0 && e0 + e < V) E::store(dx, o0 + e0 + e, 0.0f);
-    }
-  }
-}
-
-template <int DT>
-__device__ __forceinline__ void sparse_row(const char *xr, void *dx, long long o0, int V, int vb, int ve,
-                                           int shift, float mref, float l2s, float A, float B, float c,
-                                           const int *s_id, const float *s_val, int n) {
-  typedef Elem<DT> E;
-  for (int j = threadIdx.x; j < n; j += THREADS) {
-    const int id = s_id[j];
-    if (id < 0 || id >= V) continue;
-    const int vi = (int)(((long long)id + shift) / E::VEC);
-    if (vi < vb || vi >= ve) continue;
-    bool seen = false;
-    for (int i = 0; i < j; ++i) seen |= s_id[i] == id;
-    if (seen) continue;
-    float sum = 0.0f;
-    for (int i = j; i < n; ++i)
-      if (s_id[i] == id) sum += s_val[i];
-    const float d = (E::load(xr, id) - mref) * c - l2s;
-    E::store(dx, o0 + id, exp2_(d) * __builtin_fmaf(B, fmaxf(d, D_MIN), A) + sum);
-  }
-}
-
+// A group of G waves loads its stretch of the row (U vectors a lane), reads the entries while the loads
+// are under way, writes the dense part; then the first entry of every word in the stretch recomputes that
+// element with all entries of the same word added, in slot order, and stores it again (rounded once; no
+// atomics).
 struct GradArgs {
   s2c_logits lg;
   const float *stats;
   void *dx;
-  int segs, vps;         // stretches per row, vectors per stretch
+  int segs;              // stretches per row, of 64 G U vectors
   // scores
   const long long *token, *top_ids;
   const float *g_logp, *g_entropy, *g_top;
@@ -524,64 +602,112 @@ struct GradArgs {
   int K, teacher_dtype;
 };
 
-template <int DT, bool DISTILL>
-__global__ __launch_bounds__(THREADS) void vocab_bwd_kernel(GradArgs a) {
-  __shared__ int s_id[SLOTS];
-  __shared__ float s_val[SLOTS];
+template <int G>
+__device__ __forceinline__ void group_sync() {
+  if (G == 1) wave_lds_fence(); else __syncthreads();
+}
+
+template <int DT, int G, bool DISTILL>
+__global__ __launch_bounds__(256) void vocab_bwd_kernel(GradArgs a) {
+  typedef Elem<DT> E;
+  constexpr int VEC = E::VEC, GROUPS = 4 / G, LANES = 64 * G;
   static_assert(SLOTS >= KMAX + 1, "entries of a row");
-  const int tid = threadIdx.x;
+  __shared__ int s_ids[GROUPS][SLOTS];
+  __shared__ float s_vals[GROUPS][SLOTS];
+  const int grp = G == 1 ? (int)(threadIdx.x >> 6) : 0, tid = G == 1 ? lane_id() : (int)threadIdx.x;
+  int *s_id = s_ids[grp];
+  float *s_val = s_vals[grp];
   const float c = a.lg.inv_t * LOG2E, it = a.lg.inv_t;
   const int V = a.lg.V;
   const long long units = (long long)a.lg.rows * a.segs;
-  for (long long un = blockIdx.x; un < units; un += gridDim.x) {
-    const int r = (int)(un / a.segs), seg = (int)(un % a.segs);
-    const char *xr = row_ptr(a.lg, Elem<DT>::ES, r);
+  for (long long un = (long long)blockIdx.x * GROUPS + grp; un < units; un += (long long)gridDim.x * GROUPS) {
+    // last rows first: the forward pass has left them in the 256 MB cache
+    const int r = a.lg.rows - 1 - (int)(un / a.segs), seg = (int)(un % a.segs);
+    const char *xr = row_ptr(a.lg, E::ES, r);
     const long long o0 = (long long)r * V;
-    const int shift = (int)((((uintptr_t)a.dx / Elem<DT>::ES) + o0) & (Elem<DT>::VEC - 1));
-    const int nvec = (int)(((long long)V + shift + Elem<DT>::VEC - 1) / Elem<DT>::VEC);
-    const int vb = seg * a.vps, ve = min(nvec, vb + a.vps);
+    const int shift = (int)((((uintptr_t)a.dx / E::ES) + o0) & (VEC - 1));       // of the stores
     const float4 st = *reinterpret_cast<const float4 *>(a.stats + 4 * (size_t)r);
     const float mref = st.x, l2s = st.y;
-    if (l2s == INFINITY) {
-      zero_row<DT>(a.dx, o0, V, vb, ve, shift);
-      continue;
+    const bool dead = l2s == INFINITY;
+    const long long b0 = (long long)seg * LANES * U * VEC - shift;               // the stretch's first element
+    Raw x[U];
+    if (!dead) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const long long e0 = b0 + (long long)(u * LANES + tid) * VEC;
+        if (e0 >= 0 && e0 + VEC <= V) {
+          x[u] = load16<DT>(xr, e0);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[u].w[i] = 0;
+          if (e0 > -VEC && e0 < V) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+              if (e0 + e >= 0 && e0 + e < V) E::put(x[u], e, E::bits(xr, e0 + e));
+          }
+        }
+      }
     }
-    float A, B;
+    float A = 0.0f, B = 0.0f;
     int n = 0;
-    if (DISTILL) {
-      n = a.K;
-      const float g = a.g_loss[r] * it;
-      for (int j = tid; j < n; j += THREADS) {
-        const long long id = a.ids[(size_t)r * n + j];
-        s_id[j] = id < 0 ? -1 : (int)(id < V ? id : -1);
-        s_val[j] = id < 0 ? 0.0f
-                          : -g * exp2_((load_any(a.teacher, (long long)r * n + j, a.teacher_dtype) - st.z) * c - st.w);
+    if (!dead) {
+      if (DISTILL) {
+        n = a.K;
+        A = a.g_loss[r] * it;
+        for (int j = tid; j < n; j += LANES) {
+          const long long id = a.ids[(size_t)r * n + j];
+          s_id[j] = id >= 0 && id < V ? (int)id : -1;
+          s_val[j] = id < 0 ? 0.0f
+                            : -A * exp2_((load_any(a.teacher, (long long)r * n + j, a.teacher_dtype) - st.z) * c - st.w);
+        }
+      } else {
+        const float g = (a.g_logp && a.token) ? a.g_logp[r] : 0.0f;
+        const float ge = a.g_entropy ? a.g_entropy[r] : 0.0f;
+        const int k = a.g_top ? a.k : 0;
+        n = k + 1;
+        for (int j = tid; j < n; j += LANES) {
+          const long long id = j == 0 ? (a.token ? a.token[r] : -1) : a.top_ids[(size_t)r * k + j - 1];
+          s_id[j] = id >= 0 && id < V ? (int)id : -1;
+          s_val[j] = (j == 0 ? g : a.g_top[(size_t)r * k + j - 1]) * it;
+        }
+        A = -(ge * st.z * it);
+        B = -ge * LN2 * it;
       }
-      __syncthreads();
-      A = g;
-      B = 0.0f;
-    } else {
-      const float g = (a.g_logp && a.token) ? a.g_logp[r] : 0.0f;
-      const float ge = a.g_entropy ? a.g_entropy[r] : 0.0f;
-      const int k = a.g_top ? a.k : 0;
-      n = k + 1;
-      if (tid == 0) {
-        s_id[0] = a.token ? (int)a.token[r] : -1;
-        s_val[0] = g * it;
-      } else if (tid <= k) {
-        s_id[tid] = (int)a.top_ids[(size_t)r * k + tid - 1];
-        s_val[tid] = a.g_top[(size_t)r * k + tid - 1] * it;
-      }
-      __syncthreads();
-      float sum = 0.0f;
-      for (int j = 0; j < n; ++j) sum += s_val[j];
-      A = -(sum + ge * st.z * it);
-      B = -ge * LN2 * it;
     }
-    dense_row<DT>(xr, a.dx, o0, V, vb, ve, shift, mref, l2s, A, B, c);
-    __syncthreads();
-    sparse_row<DT>(xr, a.dx, o0, V, vb, ve, shift, mref, l2s, A, B, c, s_id, s_val, n);
-    __syncthreads();
+    group_sync<G>();
+    if (!DISTILL)
+      for (int j = 0; j < n; ++j) A -= s_val[j];
+    auto grad = [&](float v) {
+      const float d = (v - mref) * c - l2s;
+      return exp2_(d) * __builtin_fmaf(B, fmaxf(d, D_MIN), A);
+    };
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const long long e0 = b0 + (long long)(u * LANES + tid) * VEC;
+      float f[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) f[e] = dead ? 0.0f : grad(E::at(x[u], e));
+      if (e0 >= 0 && e0 + VEC <= V) {
+        store16<DT>(a.dx, o0 + e0, E::pack(f));
+      } else if (e0 > -VEC && e0 < V) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+          if (e0 + e >= 0 && e0 + e < V) E::store(a.dx, o0 + e0 + e, f[e]);
+      }
+    }
+    group_sync<G>();
+    for (int j = tid; j < n; j += LANES) {
+      const int id = s_id[j];
+      if (id < 0 || id < b0 || id >= b0 + (long long)LANES * U * VEC) continue;
+      bool seen = false;
+      for (int i = 0; i < j; ++i) seen |= s_id[i] == id;
+      if (seen) continue;
+      float sum = 0.0f;
+      for (int i = j; i < n; ++i)
+        if (s_id[i] == id) sum += s_val[i];
+      E::store(a.dx, o0 + id, grad(E::load(xr, id)) + sum);
+    }
+    group_sync<G>();
   }
 }
 
@@ -601,22 +727,78 @@ bool bad_logits(const s2c_logits &l) {
          ((uintptr_t)l.x & (l.dtype == S2C_F32 ? 3 : 1));
 }
 
-constexpr int MAX_GRID = 1 << 22;       // workgroups of 256: below 2^32 work-items
+constexpr int MAX_GRID = 1 << 21;       // workgroups of up to 1024: below 2^32 work-items
 
 int grid_of(long long units) { return (int)(units < MAX_GRID ? units : MAX_GRID); }
 
+// fn<element type>(), by the run-time code
+template <class F>
+void by_type(int dtype, F f) {
+  if (dtype == S2C_F32) f(std::integral_constant<int, S2C_F32>());
+  else if (dtype == S2C_BF16) f(std::integral_constant<int, S2C_BF16>());
+  else f(std::integral_constant<int, S2C_F16>());
+}
+
+long long vectors(int V, int dtype) {                  // of a row, at any alignment
+  const int vec = dtype == S2C_F32 ? 4 : 8;
+  return ((long long)V + 2 * vec - 2) / vec;
+}
+
+// How a row is shared out: `waves` of a workgroup to a stretch, `split` stretches to a row.
+//  * many rows: a wave each -- no barrier, no merge, one threshold for the whole row (59392 rows of 3500
+//    fp32 words, 5 alternatives: 161 us, against 292 us with 4 waves a row);
+//  * rows that would leave most of the chip empty: 16 waves (32768 bf16 words, one row: 8.0 us, 9.7 with 4,
+//    20.9 with 1), and stretches of at least one round of tiles, up to 256 workgroups, joined by a second
+//    launch (64 rows of 131072 words: 17.4 us in 4 stretches, 18.6 in one; one row of 262144 fp32 words: 14.2
+//    in 16, 25.5 in one);
+//  * 4 waves between (512 rows of 32000 words: 15.5 us, 34.4 with 1, 20.4 with 16) and for short rows (248
+//    rows of 3500: 5.1 us, 5.3 with 16).
+struct Plan { int waves, split; };
+
+Plan forward_plan(int rows, int V, int dtype) {
+  const long long nvec = vectors(V, dtype);
+  Plan p = {4, 1};
+  if (rows >= 2048) {
+    p.waves = 1;
+  } else if (rows < 256 && nvec > 1024) {
+    p.waves = 16;
+    while (p.split < MAX_SPLIT && 2LL * p.split * rows <= 256 && 2LL * p.split * (16 * 64 * 4) <= nvec) p.split *= 2;
+  }
+  return p;
+}
+
+template <class F>
+void by_plan(const Plan &p, F f) {
+  if (p.waves == 16) f(std::integral_constant<int, 16>());
+  else if (p.waves == 4) f(std::integral_constant<int, 4>());
+  else f(std::integral_constant<int, 1>());
+}
+
+long long split_bytes(int rows, int split, int k) {
+  return split == 1 ? 0 : (long long)rows * split * (sizeof(Stat) + 8LL * k) + 8;
+}
+
+Split split_of(const Plan &p, int rows, int k, void *ws) {
+  Split sp = {p.split, nullptr, nullptr};
+  sp.keys = (u64 *)ws;
+  sp.part = (Stat *)((char *)ws + 8LL * rows * p.split * k);
+  return sp;
+}
+
 template <bool DISTILL>
 int backward(GradArgs &a, const char *what, hipStream_t st) {
-  const int vec = a.lg.dtype == S2C_F32 ? 4 : 8;
-  const long long nvec = ((long long)a.lg.V + 2 * vec - 2) / vec;      // at any alignment
-  a.vps = 4 * THREADS;
-  a.segs = (int)((nvec + a.vps - 1) / a.vps);
-  const dim3 grid(grid_of((long long)a.lg.rows * a.segs)), block(THREADS);
-  if (a.lg.dtype == S2C_F32) hipLaunchKernelGGL((vocab_bwd_kernel<S2C_F32, DISTILL>), grid, block, 0, st, a);
-  else if (a.lg.dtype == S2C_BF16) hipLaunchKernelGGL((vocab_bwd_kernel<S2C_BF16, DISTILL>), grid, block, 0, st, a);
-  else hipLaunchKernelGGL((vocab_bwd_kernel<S2C_F16, DISTILL>), grid, block, 0, st, a);
+  const long long nvec = vectors(a.lg.V, a.lg.dtype);
+  const int G = nvec <= 64 * U ? 1 : 4;
+  a.segs = (int)((nvec + 64 * G * U - 1) / (64 * G * U));
+  const long long units = (long long)a.lg.rows * a.segs;
+  by_type(a.lg.dtype, [&](auto dt) {
+    if (G == 1) hipLaunchKernelGGL((vocab_bwd_kernel<dt.value, 1, DISTILL>), dim3(grid_of((units + 3) / 4)), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((vocab_bwd_kernel<dt.value, 4, DISTILL>), dim3(grid_of(units)), dim3(256), 0, st, a);
+  });
   return launched(what);
 }
+
+bool bad_workspace(const void *ws) { return !ws || ((uintptr_t)ws & 7); }
 
 bool bad_scores(const s2c_token_scores_args *a) {
   return !a || bad_logits(a->lg) || a->k < 0 || a->k > KMAX || a->k > a->lg.V || (a->k && !a->top_ids) ||
@@ -635,16 +817,30 @@ extern "C" long long s2c_words_args_sizeof(int which) {
          : which == 2 ? sizeof(s2c_distill_args) : 0;
 }
 
-extern "C" long long s2c_token_scores_workspace_bytes(int, int, int, int) { return 0; }
+extern "C" long long s2c_token_scores_workspace_bytes(int rows, int V, int dtype, int k) {
+  return split_bytes(rows, forward_plan(rows, V, dtype).split, k);
+}
 
 extern "C" int s2c_token_scores_fwd(const s2c_token_scores_args *a, void *stream) {
   if (bad_scores(a) || !a->entropy || (a->token && !a->logp) || (a->k && !a->top_logp)) return S2C_EINVAL;
-  if (a->lg.rows == 0) return 0;
-  const dim3 grid(grid_of(a->lg.rows)), block(THREADS);
+  const int rows = a->lg.rows;
+  if (rows == 0) return 0;
+  const Plan p = forward_plan(rows, a->lg.V, a->lg.dtype);
+  if (p.split > 1 && bad_workspace(a->ws)) return S2C_EINVAL;
+  const Split sp = split_of(p, rows, a->k, a->ws);
+  const long long units = (long long)rows * p.split;
   hipStream_t st = (hipStream_t)stream;
-  if (a->lg.dtype == S2C_F32) hipLaunchKernelGGL(scores_fwd_kernel<S2C_F32>, grid, block, 0, st, *a);
-  else if (a->lg.dtype == S2C_BF16) hipLaunchKernelGGL(scores_fwd_kernel<S2C_BF16>, grid, block, 0, st, *a);
-  else hipLaunchKernelGGL(scores_fwd_kernel<S2C_F16>, grid, block, 0, st, *a);
+  by_type(a->lg.dtype, [&](auto dt) {
+    auto go = [&](auto g) {
+      typedef Shape<g.value> Sh;
+      const dim3 grid(grid_of((units + Sh::GROUPS - 1) / Sh::GROUPS)), block(Sh::THREADS);
+      if (a->k) hipLaunchKernelGGL((scores_fwd_kernel<dt.value, g.value, true>), grid, block, 0, st, *a, sp);
+      else hipLaunchKernelGGL((scores_fwd_kernel<dt.value, g.value, false>), grid, block, 0, st, *a, sp);
+    };
+    by_plan(p, go);
+    if (p.split > 1)
+      hipLaunchKernelGGL((scores_join_kernel<dt.value>), dim3(grid_of((rows + 3LL) / 4)), dim3(256), 0, st, *a, sp);
+  });
   return launched("token_scores_fwd");
 }
 
@@ -665,16 +861,29 @@ extern "C" int s2c_token_scores_bwd(const s2c_token_scores_args *a, const float 
   return backward<false>(g, "token_scores_bwd", (hipStream_t)stream);
 }
 
-extern "C" long long s2c_distill_workspace_bytes(int, int, int) { return 0; }
+extern "C" long long s2c_distill_workspace_bytes(int rows, int V, int dtype) {
+  return split_bytes(rows, forward_plan(rows, V, dtype).split, 0);
+}
 
 extern "C" int s2c_distill_fwd(const s2c_distill_args *a, void *stream) {
   if (bad_distill(a) || !a->loss) return S2C_EINVAL;
-  if (a->lg.rows == 0) return 0;
-  const dim3 grid(grid_of(a->lg.rows)), block(THREADS);
+  const int rows = a->lg.rows;
+  if (rows == 0) return 0;
+  const Plan p = forward_plan(rows, a->lg.V, a->lg.dtype);
+  if (p.split > 1 && bad_workspace(a->ws)) return S2C_EINVAL;
+  const Split sp = split_of(p, rows, 0, a->ws);
+  const long long units = (long long)rows * p.split;
   hipStream_t st = (hipStream_t)stream;
-  if (a->lg.dtype == S2C_F32) hipLaunchKernelGGL(distill_fwd_kernel<S2C_F32>, grid, block, 0, st, *a);
-  else if (a->lg.dtype == S2C_BF16) hipLaunchKernelGGL(distill_fwd_kernel<S2C_BF16>, grid, block, 0, st, *a);
-  else hipLaunchKernelGGL(distill_fwd_kernel<S2C_F16>, grid, block, 0, st, *a);
+  by_type(a->lg.dtype, [&](auto dt) {
+    auto go = [&](auto g) {
+      typedef Shape<g.value> Sh;
+      hipLaunchKernelGGL((distill_fwd_kernel<dt.value, g.value>),
+                         dim3(grid_of((units + Sh::GROUPS - 1) / Sh::GROUPS)), dim3(Sh::THREADS), 0, st, *a, sp);
+    };
+    by_plan(p, go);
+    if (p.split > 1)
+      hipLaunchKernelGGL((distill_join_kernel<dt.value>), dim3(grid_of((rows + 3LL) / 4)), dim3(256), 0, st, *a, sp);
+  });
   return launched("distill_fwd");
 }
 

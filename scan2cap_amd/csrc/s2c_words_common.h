@@ -21,7 +21,9 @@ template <> struct Elem<S2C_F32> {
   typedef float T;
   static constexpr int VEC = 4, ES = 4;
   static constexpr u32 NEG_INF = 0xFF800000u;
-  static __device__ __forceinline__ float at(const Raw &r, int e) { return __builtin_bit_cast(float, r.w[e]); }
+  // element e of a vector, given the word that holds it
+  static __device__ __forceinline__ float of(u32 w, int) { return __builtin_bit_cast(float, w); }
+  static __device__ __forceinline__ float at(const Raw &r, int e) { return of(r.w[e], e); }
   static __device__ __forceinline__ float load(const void *p, long long i) { return ((const float *)p)[i]; }
   static __device__ __forceinline__ void store(void *p, long long i, float v) { ((float *)p)[i] = v; }
   static __device__ __forceinline__ u32 bits(const void *p, long long i) { return ((const u32 *)p)[i]; }
@@ -37,9 +39,10 @@ template <> struct Elem<S2C_BF16> {
   typedef u16 T;
   static constexpr int VEC = 8, ES = 2;
   static constexpr u32 NEG_INF = 0xFF80FF80u;
-  static __device__ __forceinline__ float at(const Raw &r, int e) {
-    return __builtin_bit_cast(float, (e & 1) ? (r.w[e >> 1] & 0xFFFF0000u) : (r.w[e >> 1] << 16));
+  static __device__ __forceinline__ float of(u32 w, int e) {
+    return __builtin_bit_cast(float, (e & 1) ? (w & 0xFFFF0000u) : (w << 16));
   }
+  static __device__ __forceinline__ float at(const Raw &r, int e) { return of(r.w[e >> 1], e); }
   static __device__ __forceinline__ float load(const void *p, long long i) {
     return __builtin_bit_cast(float, (u32)((const u16 *)p)[i] << 16);
   }
@@ -62,9 +65,10 @@ template <> struct Elem<S2C_F16> {
   typedef u16 T;
   static constexpr int VEC = 8, ES = 2;
   static constexpr u32 NEG_INF = 0xFC00FC00u;
-  static __device__ __forceinline__ float at(const Raw &r, int e) {
-    return (float)__builtin_bit_cast(_Float16, (u16)((e & 1) ? (r.w[e >> 1] >> 16) : (r.w[e >> 1] & 0xFFFFu)));
+  static __device__ __forceinline__ float of(u32 w, int e) {
+    return (float)__builtin_bit_cast(_Float16, (u16)((e & 1) ? (w >> 16) : (w & 0xFFFFu)));
   }
+  static __device__ __forceinline__ float at(const Raw &r, int e) { return of(r.w[e >> 1], e); }
   static __device__ __forceinline__ float load(const void *p, long long i) { return (float)((const _Float16 *)p)[i]; }
   static __device__ __forceinline__ void store(void *p, long long i, float v) { ((_Float16 *)p)[i] = (_Float16)v; }
   static __device__ __forceinline__ u32 bits(const void *p, long long i) { return ((const u16 *)p)[i]; }
@@ -99,16 +103,30 @@ __device__ __forceinline__ float load_any(const void *p, long long i, int dt) {
                        : dt == S2C_BF16 ? Elem<S2C_BF16>::load(p, i) : Elem<S2C_F16>::load(p, i);
 }
 
+// reductions over a wave: within rows of 16 lanes through DPP (no LDS round trips), then the four rows;
+// always in the same order
+template <int CTRL>
+__device__ __forceinline__ float dpp_f32(float v) {
+  const int i = __builtin_bit_cast(int, v);
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(i, i, CTRL, 0xF, 0xF, false));
+}
+__device__ __forceinline__ float lane_f32(float v, int lane) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+}
 __device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-  for (int k = 32; k > 0; k >>= 1) v += __shfl_xor(v, k);
-  return v;
+  v += dpp_f32<DPP_QUAD_1032>(v);
+  v += dpp_f32<DPP_QUAD_2301>(v);
+  v += dpp_f32<DPP_ROW_HALF_MIRROR>(v);
+  v += dpp_f32<DPP_ROW_MIRROR>(v);
+  return (lane_f32(v, 0) + lane_f32(v, 16)) + (lane_f32(v, 32) + lane_f32(v, 48));
 }
 // (a NaN is passed over, as fmaxf does)
 __device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int k = 32; k > 0; k >>= 1) v = fmaxf(v, __shfl_xor(v, k));
-  return v;
+  v = fmaxf(v, dpp_f32<DPP_QUAD_1032>(v));
+  v = fmaxf(v, dpp_f32<DPP_QUAD_2301>(v));
+  v = fmaxf(v, dpp_f32<DPP_ROW_HALF_MIRROR>(v));
+  v = fmaxf(v, dpp_f32<DPP_ROW_MIRROR>(v));
+  return fmaxf(fmaxf(lane_f32(v, 0), lane_f32(v, 16)), fmaxf(lane_f32(v, 32), lane_f32(v, 48)));
 }
 // order LDS accesses of the lanes of ONE wave (its LDS operations execute in order; this keeps the
 // compiler from moving them)
