@@ -89,7 +89,7 @@ int s2c_embed_fwd(long long N, int V, int D, int dtype, long long ld, const long
 /* d_table (V, D) contiguous, every row written: scale * sum of g (N rows, row stride ldg) over the
  * places of each word, in their order, held in 32 bits and rounded once; padding and bad tokens
  * contribute nothing.  Same inputs, same bits.
- * ws: s2c_embed_grad_workspace_bytes(N, V, D) bytes, 8-byte aligned (may be 0). */
+ * ws: s2c_embed_grad_workspace_bytes(N, V, D) bytes, 16-byte aligned (may be 0).  N < 2^31. */
 long long s2c_embed_grad_workspace_bytes(long long N, int V, int D);
 int s2c_embed_grad(long long N, int V, int D, int dtype, long long ldg, const long long *token,
                    const void *g, float scale, long long padding, void *d_table, void *ws,

@@ -377,6 +377,7 @@ def embed_tokens(tokens, table, scale=1.0, padding_idx=None):
     s = float(scale)
     _check(math.isfinite(s) and abs(s) <= 3e38, "scale must be finite, not %r", scale)
     _check_ids("tokens", tokens)
+    _check(tokens.numel() < 2 ** 31, "tokens: more than 2^31")
     _check_gpu(table=table, tokens=tokens)
     tokens = _ids(tokens)
     return _EmbedTokens.apply(tokens, table, s, _NONE if padding_idx is None else int(padding_idx))
