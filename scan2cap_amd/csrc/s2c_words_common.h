@@ -97,6 +97,13 @@ __device__ __forceinline__ void store16(void *p, long long i, const Raw &r) {
   *reinterpret_cast<B *>((char *)p + i * Elem<DT>::ES) = b;
 }
 
+// a 16-byte aligned store that does not stay in the caches
+__device__ __forceinline__ void store16_past_cache(void *p, long long byte, const Raw &r) {
+  typedef u32 u32x4 __attribute__((ext_vector_type(4)));
+  const u32x4 v = {r.w[0], r.w[1], r.w[2], r.w[3]};
+  __builtin_nontemporal_store(v, reinterpret_cast<u32x4 *>((char *)p + byte));
+}
+
 // element i of an array whose type is known at run time only
 __device__ __forceinline__ float load_any(const void *p, long long i, int dt) {
   return dt == S2C_F32 ? Elem<S2C_F32>::load(p, i)
