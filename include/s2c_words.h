@@ -37,7 +37,8 @@ typedef struct {
  *             order, equal ones in ascending index order, a NaN above everything
  * A row whose token equals `ignore` (has_ignore != 0) is not read: logp = entropy = top_logp = 0,
  * top_ids = -1.  A row without a finite logit (all -inf): logp = -inf, entropy = 0.  A token outside
- * [0, V): logp = NaN.  stats (rows x 4 floats) is what the backward needs.
+ * [0, V): logp = NaN.  stats (rows x 4 floats; NULL where no backward
+ * follows) is what the backward needs.
  * ws: s2c_token_scores_workspace_bytes(rows, V, dtype, k) bytes, 8-byte aligned (may be 0). */
 typedef struct {
   s2c_logits lg;
@@ -64,7 +65,7 @@ int s2c_token_scores_bwd(const s2c_token_scores_args *a, const float *g_logp, co
  *   loss = sum_j q_j (log q_j - log p[id_j]),   p = softmax(x * inv_t) over all V words.
  * mask (rows bytes, may be NULL): rows with 0 are not read.  Masked rows and rows without a used slot:
  * loss 0, zero gradient.  A row of only -inf logits: loss +inf, zero gradient.  An id >= V: NaN.
- * stats (rows x 4) as above. */
+ * stats (rows x 4, or NULL) as above. */
 typedef struct {
   s2c_logits lg;
   int K, teacher_dtype;

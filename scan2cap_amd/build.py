@@ -98,6 +98,36 @@ def build(force=False, verbose=False, contract=None):
     return out
 
 
+# The word operators' torch binding (csrc/s2c_words_torch.cpp -> lib/s2c_words_ext.so): host code over
+# libs2c_hip.so's C ABI, compiled against torch's headers.
+EXT_PATH = os.path.join(LIB_DIR, "s2c_words_ext.so")
+
+
+def build_ext(force=False, verbose=False):
+    """Compile the binding; libs2c_hip.so must be built (it is linked against it)."""
+    src = os.path.join(CSRC, "s2c_words_torch.cpp")
+    deps = [src, LIB_PATH] + glob.glob(os.path.join(_HERE, "..", "include", "*.h"))
+    if not force and os.path.exists(EXT_PATH) and \
+            all(os.path.getmtime(d) <= os.path.getmtime(EXT_PATH) for d in deps):
+        return EXT_PATH
+    import sysconfig
+    import torch
+    t = os.path.dirname(torch.__file__)
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
+           "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_EXTENSION_NAME=s2c_words_ext",
+           "-D_GLIBCXX_USE_CXX11_ABI=%d" % int(torch._C._GLIBCXX_USE_CXX11_ABI)]
+    cmd += ["-isystem" + d for d in (os.path.join(t, "include"),
+                                     os.path.join(t, "include", "torch", "csrc", "api", "include"),
+                                     os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "include"),
+                                     sysconfig.get_paths()["include"])]
+    cmd += [src, "-o", EXT_PATH, "-L" + LIB_DIR, "-ls2c_hip", "-Wl,-rpath,$ORIGIN", "-L" + os.path.join(t, "lib"),
+            "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch", "-ltorch_python"]
+    if verbose:
+        print(" ".join(cmd), file=sys.stderr)
+    subprocess.check_call(cmd)
+    return EXT_PATH
+
+
 PROBES_DIR = os.path.join(_HERE, "..", "tools", "probes")
 PROBES_PATH = os.path.join(PROBES_DIR, "libs2c_probes.so")
 
@@ -117,3 +147,5 @@ def build_probes(force=False):
 
 if __name__ == "__main__":
     print(build(force="--force" in sys.argv, verbose=True))
+    if CONTRACT == 0:
+        print(build_ext(force="--force" in sys.argv, verbose=True))

@@ -367,7 +367,7 @@ __device__ __forceinline__ void scores_write_dead(const s2c_token_scores_args &a
   if (lane == 0) {
     if (a.logp) a.logp[r] = 0.0f;
     a.entropy[r] = 0.0f;
-    *reinterpret_cast<float4 *>(a.stats + 4 * (size_t)r) = make_float4(0.0f, INFINITY, 0.0f, 0.0f);
+    if (a.stats) *reinterpret_cast<float4 *>(a.stats + 4 * (size_t)r) = make_float4(0.0f, INFINITY, 0.0f, 0.0f);
   }
   for (int j = lane; j < a.k; j += 64) {
     a.top_logp[(size_t)r * a.k + j] = 0.0f;
@@ -391,7 +391,7 @@ __device__ __forceinline__ void scores_write(const s2c_token_scores_args &a, int
       a.logp[r] = bad ? NAN : (Elem<DT>::load(xr, bad ? 0 : t) - mref) * a.lg.inv_t - LN2 * sub;
     }
     a.entropy[r] = h < 0.0f ? 0.0f : h;
-    *reinterpret_cast<float4 *>(a.stats + 4 * (size_t)r) =
+    if (a.stats) *reinterpret_cast<float4 *>(a.stats + 4 * (size_t)r) =
         make_float4(mref, bad ? NAN : l2s, h < 0.0f ? 0.0f : h, 0.0f);
   }
   if (lane < a.k) {
@@ -489,7 +489,7 @@ __device__ __forceinline__ Slots load_slots(const s2c_distill_args &a, int r, fl
 __device__ __forceinline__ void distill_write_dead(const s2c_distill_args &a, int r, int lane) {
   if (lane == 0) {
     a.loss[r] = 0.0f;
-    *reinterpret_cast<float4 *>(a.stats + 4 * (size_t)r) = make_float4(0.0f, INFINITY, 0.0f, INFINITY);
+    if (a.stats) *reinterpret_cast<float4 *>(a.stats + 4 * (size_t)r) = make_float4(0.0f, INFINITY, 0.0f, INFINITY);
   }
 }
 
@@ -519,7 +519,7 @@ __device__ __forceinline__ void distill_write(const s2c_distill_args &a, int r, 
   bad = __ballot(bad) != 0;
   if (lane == 0) {
     a.loss[r] = bad ? NAN : part;
-    *reinterpret_cast<float4 *>(a.stats + 4 * (size_t)r) = make_float4(mref, bad ? NAN : l2s, t.wm, t.l2w);
+    if (a.stats) *reinterpret_cast<float4 *>(a.stats + 4 * (size_t)r) = make_float4(mref, bad ? NAN : l2s, t.wm, t.l2w);
   }
 }
 
@@ -839,13 +839,12 @@ int backward(GradArgs &a, const char *what, hipStream_t st) {
 bool bad_workspace(const void *ws) { return !ws || ((uintptr_t)ws & 7); }
 
 bool bad_scores(const s2c_token_scores_args *a) {
-  return !a || bad_logits(a->lg) || a->k < 0 || a->k > KMAX || a->k > a->lg.V || (a->k && !a->top_ids) ||
-         !a->stats;
+  return !a || bad_logits(a->lg) || a->k < 0 || a->k > KMAX || a->k > a->lg.V || (a->k && !a->top_ids);
 }
 
 bool bad_distill(const s2c_distill_args *a) {
   return !a || bad_logits(a->lg) || a->K <= 0 || a->K > SLOTS || a->teacher_dtype < 0 ||
-         a->teacher_dtype > 2 || !a->ids || !a->teacher || !a->stats;
+         a->teacher_dtype > 2 || !a->ids || !a->teacher;
 }
 
 }  // namespace
@@ -884,7 +883,7 @@ extern "C" int s2c_token_scores_fwd(const s2c_token_scores_args *a, void *stream
 
 extern "C" int s2c_token_scores_bwd(const s2c_token_scores_args *a, const float *g_logp,
                                     const float *g_entropy, const float *g_top, void *dx, void *stream) {
-  if (bad_scores(a) || !dx) return S2C_EINVAL;
+  if (bad_scores(a) || !a->stats || !dx) return S2C_EINVAL;
   if (a->lg.rows == 0) return 0;
   GradArgs g = {};
   g.lg = a->lg;
@@ -926,7 +925,7 @@ extern "C" int s2c_distill_fwd(const s2c_distill_args *a, void *stream) {
 }
 
 extern "C" int s2c_distill_bwd(const s2c_distill_args *a, const float *g_loss, void *dx, void *stream) {
-  if (bad_distill(a) || !g_loss || !dx) return S2C_EINVAL;
+  if (bad_distill(a) || !a->stats || !g_loss || !dx) return S2C_EINVAL;
   if (a->lg.rows == 0) return 0;
   GradArgs g = {};
   g.lg = a->lg;
