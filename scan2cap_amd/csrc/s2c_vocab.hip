@@ -126,6 +126,12 @@ struct Best {
   }
 };
 
+// what the waves of a group share: their lane maxima, the number of their candidates
+struct Shared {
+  u32 max[64];
+  int n;
+};
+
 // the k best of L (a power of two <= 64) sorted lists, key(list, pos); 64 / L places of every list at a
 // time, so that a round that adds nothing ends it.  b.buf holds them in descending order afterwards.
 template <class F>
@@ -304,7 +310,7 @@ struct Split {
 // Every wave of the workgroup comes here together where G > 1.
 template <int DT, int G, bool TOP, bool ENT>
 __device__ __forceinline__ Stat group_stat(const char *xr, int V, int seg, int segs, int k, float c,
-                                           u64 (*lists)[BUF], Stat *s_part, u32 *s_max) {
+                                           u64 (*lists)[BUF], Stat *s_part, Shared *sh) {
   typedef Elem<DT> E;
   const int lane = lane_id(), w = G == 1 ? 0 : (int)(threadIdx.x >> 6);
   const int shift = (int)(((uintptr_t)xr / E::ES) & (E::VEC - 1));
@@ -313,27 +319,44 @@ __device__ __forceinline__ Stat group_stat(const char *xr, int V, int seg, int s
   const int vb = min(nvec, seg * per), ve = min(nvec, vb + per);
   Best best;
   if (TOP) best.init(lists[w], k);
-  Stat s = stream_row<DT, G, TOP, ENT>(xr, V, vb, ve, w, c, best, s_max);
+  // (nobody counts before the barrier inside stream_row, nobody reads the last count after the one before this)
+  if (TOP && G > 1 && w == 0 && lane == 0) sh->n = 0;
+  Stat s = stream_row<DT, G, TOP, ENT>(xr, V, vb, ve, w, c, best, TOP && G > 1 ? sh->max : nullptr);
+  if (G == 1) {
+    if (TOP) best.cut(lane);
+    return s;
+  }
   if (TOP) {
+    int at = 0;
+    if (lane == 0) at = atomicAdd(&sh->n, best.cnt);
+    at = __builtin_amdgcn_readfirstlane(at);
+    if (at + best.cnt <= BUF)
+      for (int i = lane; i < best.cnt; i += 64) lists[G][at + i] = lists[w][i];
+  }
+  if (lane == 0) s_part[w] = s;
+  __syncthreads();
+  const int n = TOP ? sh->n : 0;
+  if (n > BUF) {                             // too many for one buffer: every wave's k best, sorted
     best.cut(lane);
     for (int j = best.cnt + lane; j < k; j += 64) lists[w][j] = 0;
-    wave_lds_fence();
-  }
-  if (G > 1) {
-    if (lane == 0) s_part[w] = s;
     __syncthreads();
-    if (w == 0) {
-      Stat o = {-INFINITY, 0.0f, 0.0f};
-      if (lane < G) o = s_part[lane];
-      s = wave_combine(o, c);
-      if (TOP) {
-        s_max[lane] = 0;                     // (read by all, needed again after the workgroup's next barrier)
-        Best all;
-        all.init(lists[G], k);
+  }
+  if (w == 0) {
+    Stat o = {-INFINITY, 0.0f, 0.0f};
+    if (lane < G) o = s_part[lane];
+    s = wave_combine(o, c);
+    if (TOP) {
+      sh->max[lane] = 0;                     // (read by all, needed again after the workgroup's next barrier)
+      Best all;
+      all.init(lists[G], k);
+      if (n > BUF) {
         merge_lists(all, G, lane, [&](int list, int pos) { return lists[list][pos]; });
-        for (int j = all.cnt + lane; j < k; j += 64) lists[G][j] = 0;
-        wave_lds_fence();
+      } else {
+        all.cnt = n;
+        all.cut(lane);
       }
+      for (int j = all.cnt + lane; j < k; j += 64) lists[G][j] = 0;
+      wave_lds_fence();
     }
   }
   return s;
@@ -406,12 +429,12 @@ __global__ __launch_bounds__(Shape<G>::THREADS) void scores_fwd_kernel(s2c_token
   typedef Shape<G> Sh;
   __shared__ u64 s_lists[TOP ? Sh::WAVES + (G > 1) : 1][TOP ? BUF : 1];
   __shared__ Stat s_part[Sh::WAVES];
-  __shared__ u32 s_max[64];
+  __shared__ Shared s_shared;
   const int lane = lane_id(), w = threadIdx.x >> 6;
   const int grp = G == 1 ? w : 0;
   const bool first = G == 1 || w == 0;
   if (TOP && G > 1) {
-    if (w == 0) s_max[lane] = 0;
+    if (w == 0) s_shared.max[lane] = 0;
     __syncthreads();
   }
   u64 (*lists)[BUF] = reinterpret_cast<u64 (*)[BUF]>(&s_lists[TOP ? grp : 0][0]);
@@ -424,7 +447,7 @@ __global__ __launch_bounds__(Shape<G>::THREADS) void scores_fwd_kernel(s2c_token
       continue;
     }
     const char *xr = row_ptr(a.lg, Elem<DT>::ES, r);
-    const Stat s = group_stat<DT, G, TOP, true>(xr, a.lg.V, seg, sp.n, a.k, c, lists, s_part, s_max);
+    const Stat s = group_stat<DT, G, TOP, true>(xr, a.lg.V, seg, sp.n, a.k, c, lists, s_part, &s_shared);
     if (first) {
       const u64 *list = lists[G > 1 ? G : 0];
       if (sp.n == 1) scores_write<DT>(a, r, xr, s, list, lane);
@@ -590,7 +613,7 @@ struct GradArgs {
   s2c_logits lg;
   const float *stats;
   void *dx;
-  int segs;              // stretches per row, of 64 G U vectors
+  int segs, span;        // stretches per row, of `span` vectors (64 G U at most)
   int past_cache;        // dx does not fit the cache: stored past it
   // scores
   const long long *token, *top_ids;
@@ -634,22 +657,22 @@ __global__ __launch_bounds__(256) void vocab_bwd_kernel(GradArgs a) {
     const float4 st = *reinterpret_cast<const float4 *>(a.stats + 4 * (size_t)r);
     const float mref = st.x, l2s = st.y;
     const bool dead = l2s == INFINITY;
-    const long long b0 = (long long)seg * LANES * U * VEC - shift;               // the stretch's elements
-    const long long b1 = min((long long)V, b0 + (long long)LANES * U * VEC);
+    const long long b0 = (long long)seg * a.span * VEC - shift;                  // the stretch's elements
+    const long long b1 = min((long long)V, b0 + (long long)a.span * VEC);
     Raw x[U];
     if (!dead) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         const long long e0 = b0 + (long long)(u * LANES + tid) * VEC;
-        if (e0 >= 0 && e0 + VEC <= V) {
+        if (e0 >= 0 && e0 + VEC <= b1) {
           x[u] = load16<DT>(xr, e0);
         } else {
 #pragma unroll
           for (int i = 0; i < 4; ++i) x[u].w[i] = 0;
-          if (e0 > -VEC && e0 < V) {
+          if (e0 > -VEC && e0 < b1) {
 #pragma unroll
             for (int e = 0; e < VEC; ++e)
-              if (e0 + e >= 0 && e0 + e < V) E::put(x[u], e, E::bits(xr, e0 + e));
+              if (e0 + e >= 0 && e0 + e < b1) E::put(x[u], e, E::bits(xr, e0 + e));
           }
         }
       }
@@ -718,13 +741,13 @@ __global__ __launch_bounds__(256) void vocab_bwd_kernel(GradArgs a) {
       float f[VEC];
 #pragma unroll
       for (int e = 0; e < VEC; ++e) f[e] = dead ? 0.0f : grad(E::at(x[u], e));
-      if (e0 >= 0 && e0 + VEC <= V) {
+      if (e0 >= 0 && e0 + VEC <= b1) {
         if (a.past_cache) store16_past_cache(a.dx, (o0 + e0) * E::ES, E::pack(f));
         else store16<DT>(a.dx, o0 + e0, E::pack(f));
-      } else if (e0 > -VEC && e0 < V) {
+      } else if (e0 > -VEC && e0 < b1) {
 #pragma unroll
         for (int e = 0; e < VEC; ++e)
-          if (e0 + e >= 0 && e0 + e < V) E::store(a.dx, o0 + e0 + e, f[e]);
+          if (e0 + e >= 0 && e0 + e < b1) E::store(a.dx, o0 + e0 + e, f[e]);
       }
     }
     group_sync<G>();
@@ -825,6 +848,7 @@ int backward(GradArgs &a, const char *what, hipStream_t st) {
   const long long nvec = vectors(a.lg.V, a.lg.dtype);
   const int G = nvec <= 64 * U ? 1 : 4;
   a.segs = (int)((nvec + 64 * G * U - 1) / (64 * G * U));
+  a.span = (int)((nvec + a.segs - 1) / a.segs);
   // a gradient that is larger than the 256 MB cache would leave it full of lines to be written back: the
   // next forward pass over 4096 x 50001 bf16 takes 122 us behind ordinary stores, 90 us behind these
   a.past_cache = (double)a.lg.rows * a.lg.V * (a.lg.dtype == S2C_F32 ? 4 : 2) > 256.0 * (1 << 20);
