@@ -9,12 +9,12 @@
 //  * looking through all tokens (few tokens: one launch), or
 //  * a stable sort of (word, place) by word; padding and bad tokens sort behind the last word.  The sorted
 //    order is cut into chunks, a wave each, whatever words are in them (a word's run may be most of the
-//    batch, or one place): the wave reads its rows 8 at a time and writes a word's sum when its run ends.
+//    batch, or one place): the wave has 4 to 8 of its rows under way and writes a word's sum when its run ends.
 //    A run that passes a chunk's border leaves partial sums, which a last launch joins in order; it also
 //    writes the rows of the words that are not in the batch.
-// Measured (kernel times, MI355X): 131072 tokens x 1024 bf16, 50001 words: lookup 83 us (3.9 TB/s),
-// gradient 164 us = sort 30 + runs 108 + join 26 (floor 73 us at 5.1 TB/s); 8191 x 515 fp16, 10007 words:
-// lookup 5.4 us, gradient 36 us = sort 18 + 10 + 8.
+// Measured (kernel times, MI355X): 131072 tokens x 1024 bf16, 50001 words: lookup 79 us (4.1 TB/s),
+// gradient 135 us = sort 31 + runs 79 + join 25 (floor 73 us at 5.1 TB/s); 8191 x 515 fp16, 10007 words:
+// lookup 5.6 us, gradient 35 us = sort 18 + 9 + 8.
 #include "s2c_words_common.h"
 
 #include <stdio.h>
@@ -57,7 +57,7 @@ __global__ __launch_bounds__(THREADS) void embed_fwd_kernel(long long N, int V, 
                                                             const long long *__restrict__ token,
                                                             const void *__restrict__ table, float scale,
                                                             long long padding, void *__restrict__ out,
-                                                            int lpr) {
+                                                            int lpr, bool past_cache) {
   typedef Elem<DT> E;
   const int sub = threadIdx.x & (lpr - 1), per = THREADS / lpr;
   const long long step = (long long)gridDim.x * per * ROWS;
@@ -80,7 +80,8 @@ __global__ __launch_bounds__(THREADS) void embed_fwd_kernel(long long N, int V, 
         float f[E::VEC];
 #pragma unroll
         for (int e = 0; e < E::VEC; ++e) f[e] = bad ? NAN : t[i] == padding ? 0.0f : scale * E::at(r[i], e);
-        store_part<DT>(out, n * D + c, D - c, f);
+        if (past_cache) store16_past_cache(out, (n * D + c) * E::ES, E::pack(f));
+        else store_part<DT>(out, n * D + c, D - c, f);
       }
     }
   }
@@ -360,6 +361,8 @@ __global__ __launch_bounds__(THREADS) void sort_scatter_kernel(SortArgs a) {
   }
 }
 
+constexpr int BATCH = 4;          // rows of a chunk that are asked for together
+
 // The first `sums` workgroups: the sums of the chunks' runs.  The others: start[v], the first place of word v
 // in the sorted order.
 template <int DT>
@@ -390,14 +393,21 @@ __global__ __launch_bounds__(THREADS) void embed_runs_kernel(GradArgs a, int sum
     Acc<DT> acc;
     acc.clear();
     bool began_before = n > 0 && (u32)__builtin_amdgcn_readlane((int)key, 0) == before;
-    for (int j0 = 0; j0 < n; j0 += AHEAD) {
-      Raw r[AHEAD];
+    auto row = [&](int j) {
+      return load_part<DT>(a.g, (long long)(u32)__builtin_amdgcn_readlane((int)pos, j) * a.ldg + col, a.D - col);
+    };
+    Raw r[BATCH], next[BATCH];                        // these are added while the next are under way
 #pragma unroll
-      for (int q = 0; q < AHEAD; ++q)
-        if (j0 + q < n)
-          r[q] = load_part<DT>(a.g, (long long)(u32)__builtin_amdgcn_readlane((int)pos, j0 + q) * a.ldg + col, a.D - col);
+    for (int q = 0; q < BATCH; ++q)
+      if (q < n) next[q] = row(q);
+    for (int j0 = 0; j0 < n; j0 += BATCH) {
 #pragma unroll
-      for (int q = 0; q < AHEAD; ++q) {
+      for (int q = 0; q < BATCH; ++q) r[q] = next[q];
+#pragma unroll
+      for (int q = 0; q < BATCH; ++q)
+        if (j0 + BATCH + q < n) next[q] = row(j0 + BATCH + q);
+#pragma unroll
+      for (int q = 0; q < BATCH; ++q) {
         const int j = j0 + q;
         if (j >= n) break;
         acc.add(r[q]);
@@ -524,15 +534,19 @@ extern "C" int s2c_embed_fwd(long long N, int V, int D, int dtype, long long ld,
   int lpr = 1;
   while (lpr < 64 && lpr * vec < D) lpr *= 2;
   hipStream_t st = (hipStream_t)stream;
+  // an output that the 256 MB cache cannot hold is stored past it, in whole vectors (131072 x 4096 bf16: 223 us,
+  // 262 us through it; and what runs next finds no lines to be written back)
+  const long long row_bytes = (long long)D * (dtype == S2C_F32 ? 4 : 2);
+  const bool past_cache = N * row_bytes >= (256LL << 20) && row_bytes % 16 == 0 && ((uintptr_t)out & 15) == 0;
   auto go = [&](auto dt, auto rows) {
     const long long per = (long long)THREADS / lpr * rows.value;
     hipLaunchKernelGGL((embed_fwd_kernel<dt.value, rows.value>), dim3(grid_of((N + per - 1) / per)), dim3(THREADS), 0,
-                       st, N, V, D, ld, token, table, scale, padding, out, lpr);
+                       st, N, V, D, ld, token, table, scale, padding, out, lpr, past_cache);
   };
   auto by_rows = [&](auto dt) {
-    // many short rows: a lane has 4 of them under way (10^6 rows of 512 bytes: 133 us, 153 with one); else
-    // as many waves as there are (2048 rows of 1200 bytes: 3.4 us, 4.5 with four)
-    if (lpr < 64 && N * lpr >= (1LL << 21)) go(dt, std::integral_constant<int, 4>());
+    // many rows: a lane has 4 of them under way (131072 rows of 2 KB: 58 us, 65 with one; 10^6 of 512 bytes:
+    // 133 us, 153), else as many waves as there are (32768 rows of 2 KB: 15.6 us, 17.1 with four)
+    if (N * lpr >= (1LL << 22)) go(dt, std::integral_constant<int, 4>());
     else go(dt, std::integral_constant<int, 1>());
   };
   if (dtype == S2C_F32) by_rows(std::integral_constant<int, S2C_F32>());
@@ -550,7 +564,7 @@ static long long align16(long long n) { return (n + 15) & ~15LL; }
 static int pieces_of(int D, int vec) { return (D + 64 * vec - 1) / (64 * vec); }
 
 // About 4096 waves, and 64 places (a lane each) at most: shorter chunks leave more partial sums (131072
-// rows of 1024 bf16: runs 108 + join 26 us, 98 + 90 us with four times the waves).
+// rows of 1024 bf16: runs 95 + join 25 us, 105 + 26 us with twice the waves).
 static int chunk_of(long long N, int D) {
   const long long want = N * pieces_of(D, 8) / 4096;
   return want >= 64 ? 64 : want >= 32 ? 32 : want >= 16 ? 16 : 8;

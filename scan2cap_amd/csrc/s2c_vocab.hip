@@ -849,9 +849,9 @@ int backward(GradArgs &a, const char *what, hipStream_t st) {
   const int G = nvec <= 64 * U ? 1 : 4;
   a.segs = (int)((nvec + 64 * G * U - 1) / (64 * G * U));
   a.span = (int)((nvec + a.segs - 1) / a.segs);
-  // a gradient that is larger than the 256 MB cache would leave it full of lines to be written back: the
+  // a gradient that the 256 MB cache cannot hold would leave it full of lines to be written back: the
   // next forward pass over 4096 x 50001 bf16 takes 122 us behind ordinary stores, 90 us behind these
-  a.past_cache = (double)a.lg.rows * a.lg.V * (a.lg.dtype == S2C_F32 ? 4 : 2) > 256.0 * (1 << 20);
+  a.past_cache = (double)a.lg.rows * a.lg.V * (a.lg.dtype == S2C_F32 ? 4 : 2) >= 256.0 * (1 << 20);
   const long long units = (long long)a.lg.rows * a.segs;
   by_type(a.lg.dtype, [&](auto dt) {
     if (G == 1) hipLaunchKernelGGL((vocab_bwd_kernel<dt.value, 1, DISTILL>), dim3(grid_of((units + 3) / 4)), dim3(256), 0, st, a);
