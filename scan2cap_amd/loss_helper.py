@@ -168,6 +168,70 @@ def compute_cap_loss(data_dict, config, weights):
     return cap_loss, cap_acc
 
 
+def _trained_words(data_dict):
+    """The words (B,T-1) that `lang_cap`'s teacher-forced logits are for."""
+    num_words = data_dict.get("_num_words")
+    if num_words is None:
+        num_words = int(data_dict["lang_len"].max())
+    targets = data_dict["lang_ids"][:, 1:num_words]
+    if tuple(data_dict["lang_cap"].shape[:2]) != tuple(targets.shape):
+        raise ValueError("lang_cap has %s words but the targets have %s (is data_dict['_num_words'] = %r stale?)"
+                         % (tuple(data_dict["lang_cap"].shape[:2]), tuple(targets.shape), num_words))
+    return targets
+
+
+def attach_teacher(data_dict, teacher_dict, top_k=16):
+    """Put a teacher's best alternatives for every word into `data_dict` for `compute_cap_distill_loss`:
+    `teacher_top_ids` (B,T-1,top_k) int64 and `teacher_top_logits` (their log probabilities), from the
+    `lang_cap` logits of `teacher_dict` (the same batch run through the teacher, teacher-forced)."""
+    logits = teacher_dict["lang_cap"].detach()
+    if logits.is_cuda:
+        from . import word_ops
+        best = word_ops.token_scores(logits, top_k=top_k)
+        data_dict["teacher_top_ids"], data_dict["teacher_top_logits"] = best.top_ids, best.top_logp
+    else:
+        logp = F.log_softmax(logits, -1)
+        ids = torch.sort(logits, dim=-1, descending=True, stable=True)[1][..., :top_k]
+        data_dict["teacher_top_ids"], data_dict["teacher_top_logits"] = ids, torch.gather(logp, -1, ids)
+    return data_dict
+
+
+def compute_cap_distill_loss(data_dict, temperature=2.0):
+    """Distillation of the captioner from a teacher's top logits (`attach_teacher`): temperature^2 times the
+    mean over the trained words (good boxes, not padding) of KL(teacher's top words || student's softmax), both
+    at `temperature`."""
+    logits = data_dict["lang_cap"]
+    rows = (_trained_words(data_dict) != 0) & (data_dict["good_bbox_masks"] != 0).unsqueeze(1)
+    ids, teacher = data_dict["teacher_top_ids"], data_dict["teacher_top_logits"]
+    if logits.is_cuda:
+        from . import word_ops
+        kd = word_ops.distill_loss(logits, ids, teacher.detach(), temperature=temperature, mask=rows)
+    else:
+        used = ids >= 0
+        w = (teacher.detach() / temperature).masked_fill(~used, float("-inf"))
+        live = rows & used.any(-1)
+        logq = F.log_softmax(torch.where(live.unsqueeze(-1), w, torch.zeros_like(w)), -1)
+        at = torch.gather(F.log_softmax(logits / temperature, -1), -1, ids.clamp(min=0))
+        q = logq.exp()
+        terms = torch.where(q > 0, q * (logq.clamp(min=-1e30) - at), torch.zeros_like(q))
+        kd = torch.where(live, terms.sum(-1), torch.zeros_like(terms[..., 0]))
+    return temperature ** 2 * kd.sum() / (rows.sum() + 1e-6)
+
+
+def caption_log_likelihood(data_dict, temperature=1.0):
+    """log p of the captions `lang_ids` under the teacher-forced logits `lang_cap` (for scoring and reranking):
+    (B,) sums over the words that are not padding, and (B,T-1) of every word (0 at padding)."""
+    logits = data_dict["lang_cap"]
+    targets = _trained_words(data_dict)
+    if logits.is_cuda:
+        from . import word_ops
+        logp = word_ops.token_scores(logits, targets, temperature=temperature, ignore_index=0).logp
+    else:
+        logp = torch.gather(F.log_softmax(logits / temperature, -1), -1, targets.unsqueeze(-1)).squeeze(-1)
+        logp = torch.where(targets != 0, logp, torch.zeros_like(logp))
+    return logp.sum(-1), logp
+
+
 def radian_to_label(radians, num_bins=6):
     """loss_helper.py:232-247."""
     boundaries = torch.arange(np.pi / num_bins, np.pi - 1e-8, np.pi / num_bins,
@@ -232,7 +296,7 @@ def compute_node_distance_loss(data_dict):
 
 
 def _get_scene_cap_loss_fused(data_dict, device, config, weights, detection, caption,
-                              orientation, distance, num_bins):
+                              orientation, distance, num_bins, distill, distill_temperature):
     """Same contract as below; detection terms from the fused HIP kernels."""
     det, stats, objectness_label, objectness_mask, object_assignment = \
         loss_fused.detection_loss(data_dict, config, NEAR_THRESHOLD, FAR_THRESHOLD,
@@ -267,12 +331,15 @@ def _get_scene_cap_loss_fused(data_dict, device, config, weights, detection, cap
         loss = loss + 0.1 * data_dict["ori_loss"]
     if distance:
         loss = loss + 0.1 * data_dict["dist_loss"]
+    if distill:
+        data_dict["distill_loss"] = compute_cap_distill_loss(data_dict, distill_temperature)
+        loss = loss + distill * data_dict["distill_loss"]
     data_dict["loss"] = loss
-    _publish_parts(data_dict, det if detection else None, caption, orientation, distance)
+    _publish_parts(data_dict, det if detection else None, caption, orientation, distance, distill)
     return data_dict
 
 
-def _publish_parts(data_dict, det, caption, orientation, distance):
+def _publish_parts(data_dict, det, caption, orientation, distance, distill):
     """loss = _loss_det + _loss_rest (the detector part / everything that flows through the
     relation graph and the captioner) for parallel.backward_in_two_stages."""
     rest = None
@@ -282,16 +349,21 @@ def _publish_parts(data_dict, det, caption, orientation, distance):
         rest = 0.1 * data_dict["ori_loss"] if rest is None else rest + 0.1 * data_dict["ori_loss"]
     if distance:
         rest = 0.1 * data_dict["dist_loss"] if rest is None else rest + 0.1 * data_dict["dist_loss"]
+    if distill:
+        kd = distill * data_dict["distill_loss"]
+        rest = kd if rest is None else rest + kd
     data_dict["_loss_det"], data_dict["_loss_rest"] = det, rest
 
 
 def get_scene_cap_loss(data_dict, device, config, weights, detection=True,
                        caption=True, orientation=False, distance=False,
-                       num_bins=CONF.TRAIN.NUM_BINS):
-    """loss_helper.py:381-491: same keys written into data_dict, same weights."""
+                       num_bins=CONF.TRAIN.NUM_BINS, distill=0.0, distill_temperature=2.0):
+    """loss_helper.py:381-491: same keys written into data_dict, same weights.  distill > 0 adds that much of
+    the captioner's distillation loss (`attach_teacher` first); not in the reference."""
     if FUSED_DETECTION_LOSS and loss_fused.available(data_dict):
         return _get_scene_cap_loss_fused(data_dict, device, config, weights, detection,
-                                         caption, orientation, distance, num_bins)
+                                         caption, orientation, distance, num_bins, distill,
+                                         distill_temperature)
     vote_loss = compute_vote_loss(data_dict)
     objectness_loss, objectness_label, objectness_mask, object_assignment = \
         compute_objectness_loss(data_dict)
@@ -351,6 +423,9 @@ def get_scene_cap_loss(data_dict, device, config, weights, detection=True,
         loss = loss + 0.1 * data_dict["ori_loss"]
     if distance:
         loss = loss + 0.1 * data_dict["dist_loss"]
+    if distill:
+        data_dict["distill_loss"] = compute_cap_distill_loss(data_dict, distill_temperature)
+        loss = loss + distill * data_dict["distill_loss"]
     data_dict["loss"] = loss
-    _publish_parts(data_dict, det, caption, orientation, distance)
+    _publish_parts(data_dict, det, caption, orientation, distance, distill)
     return data_dict

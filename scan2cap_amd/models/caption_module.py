@@ -149,6 +149,30 @@ def _embedding_table(vocabulary, embeddings, emb_size):
     return torch.from_numpy(table)
 
 
+def _word_embs(module, data_dict):
+    """The captions' word embeddings (B,T,emb): `lang_feat` where the caller brought it (the reference's
+    dataset looks every word up on the host, lib/dataset.py:184-199), else the table's rows of `lang_ids` on
+    the device, zeros at padding (word 0) -- 8 bytes a word to copy instead of 1200, and a gradient for a
+    table that `learn_word_embeddings` has made a parameter."""
+    if "lang_feat" in data_dict:
+        return data_dict["lang_feat"]
+    ids, table = data_dict["lang_ids"], module._emb_table
+    if table.is_cuda:
+        from ..word_ops import embed_tokens
+        return embed_tokens(ids, table, padding_idx=0)
+    return table[ids] * (ids != 0).unsqueeze(-1).to(table.dtype)
+
+
+def _learn_word_embeddings(module):
+    """Make the captioner's embedding table a parameter (`_emb_table`, in `state_dict()` from then on), so that
+    it trains with the rest when `lang_feat` is not given."""
+    if not isinstance(module._emb_table, nn.Parameter):
+        table = module._emb_table
+        del module._emb_table
+        module._emb_table = nn.Parameter(table.detach().clone())
+    return module
+
+
 _C.register("s2c_good_bbox_stats", [_I, _P, _F32, _P, _P, _P])
 
 
@@ -186,6 +210,8 @@ class SceneCaptionModule(nn.Module):
                              _embedding_table(vocabulary, embeddings, emb_size),
                              persistent=False)
 
+    learn_word_embeddings = _learn_word_embeddings
+
     def step(self, step_input, hidden):
         hidden = self.recurrent_cell(step_input, hidden)
         return hidden, hidden
@@ -198,7 +224,7 @@ class SceneCaptionModule(nn.Module):
 
     def forward_sample_batch(self, data_dict, max_len=CONF.TRAIN.MAX_DES_LEN,
                              min_iou=CONF.TRAIN.MIN_IOU_THRESHOLD):
-        word_embs = data_dict["lang_feat"]
+        word_embs = _word_embs(self, data_dict)
         B = word_embs.shape[0]
         steps = _num_words(data_dict) - 1
         obj_feats = self.map_feat(data_dict["bbox_feature"])
@@ -217,7 +243,7 @@ class SceneCaptionModule(nn.Module):
 
     def forward_scene_batch(self, data_dict, use_tf=False,
                             max_len=CONF.TRAIN.MAX_DES_LEN):
-        word_embs = data_dict["lang_feat"]
+        word_embs = _word_embs(self, data_dict)
         B = word_embs.shape[0]
         K = self.num_proposals
         steps = (_num_words(data_dict) - 1) if use_tf else (max_len - 1)
@@ -268,6 +294,8 @@ class TopDownSceneCaptionModule(nn.Module):
         self.register_buffer("_emb_table",
                              _embedding_table(vocabulary, embeddings, emb_size),
                              persistent=False)
+
+    learn_word_embeddings = _learn_word_embeddings
 
     # ---- one recurrent step ------------------------------------------------
     def _step(self, step_input, target_feat, obj_feats, hidden_1, hidden_2,
@@ -327,11 +355,13 @@ class TopDownSceneCaptionModule(nn.Module):
     # ---- training: teacher-forced decode of the target object --------------
     def _forward_sample_batch(self, data_dict, max_len=CONF.TRAIN.MAX_DES_LEN,
                               min_iou=CONF.TRAIN.MIN_IOU_THRESHOLD):
-        word_embs = data_dict["lang_feat"]          # (B,T,emb)
+        word_embs = _word_embs(self, data_dict)          # (B,T,emb)
         obj_feats = data_dict["bbox_feature"]       # (B,K,F)
         object_masks = data_dict["bbox_mask"]       # (B,K)
         B = word_embs.shape[0]
         steps = max(_num_words(data_dict) - 1, 1)
+        if word_embs.requires_grad:
+            word_embs = word_embs[:, :steps]        # (the decoder's gradient covers the words it reads)
 
         if self.use_oracle:
             target_ids = data_dict["bbox_idx"]
@@ -428,7 +458,7 @@ class TopDownSceneCaptionModule(nn.Module):
          and 8.6 GB of activations.  Values are identical up to the
         order of additions of exact zeros; the dense (B,K,K,T) attention output is
         rebuilt by scattering."""
-        word_embs = data_dict["lang_feat"]
+        word_embs = _word_embs(self, data_dict)
         obj_feats = data_dict["bbox_feature"]       # (B,K,F)
         object_masks = data_dict["bbox_mask"]
         B, K, F_ = obj_feats.shape
@@ -494,7 +524,7 @@ class TopDownSceneCaptionModule(nn.Module):
         return data_dict
 
     def _forward_scene_batch_dense(self, data_dict, max_len=CONF.TRAIN.MAX_DES_LEN):
-        word_embs = data_dict["lang_feat"]
+        word_embs = _word_embs(self, data_dict)
         obj_feats = data_dict["bbox_feature"]       # (B,K,F)
         object_masks = data_dict["bbox_mask"]
         B, K, F_ = obj_feats.shape
