@@ -37,8 +37,8 @@ typedef struct {
  *             order, equal ones in ascending index order, a NaN above everything
  * A row whose token equals `ignore` (has_ignore != 0) is not read: logp = entropy = top_logp = 0,
  * top_ids = -1.  A row without a finite logit (all -inf): logp = -inf, entropy = 0.  A token outside
- * [0, V): logp = NaN.  stats (rows x 4 floats; NULL where no backward
- * follows) is what the backward needs.
+ * [0, V): logp = NaN.  stats (rows x 4 floats, 16-byte aligned; NULL
+ * where no backward follows) is what the backward needs.
  * ws: s2c_token_scores_workspace_bytes(rows, V, dtype, k) bytes, 8-byte aligned (may be 0). */
 typedef struct {
   s2c_logits lg;

@@ -860,6 +860,11 @@ int backward(GradArgs &a, const char *what, hipStream_t st) {
   return launched(what);
 }
 
+// the gradient, and the statistics that are read 16 bytes at a time
+bool bad_backward(const s2c_logits &l, const float *stats, const void *dx) {
+  return !stats || ((uintptr_t)stats & 15) || !dx || ((uintptr_t)dx & (l.dtype == S2C_F32 ? 3 : 1));
+}
+
 bool bad_workspace(const void *ws) { return !ws || ((uintptr_t)ws & 7); }
 
 bool bad_scores(const s2c_token_scores_args *a) {
@@ -883,7 +888,9 @@ extern "C" long long s2c_token_scores_workspace_bytes(int rows, int V, int dtype
 }
 
 extern "C" int s2c_token_scores_fwd(const s2c_token_scores_args *a, void *stream) {
-  if (bad_scores(a) || !a->entropy || (a->token && !a->logp) || (a->k && !a->top_logp)) return S2C_EINVAL;
+  if (bad_scores(a) || !a->entropy || (a->token && !a->logp) || (a->k && !a->top_logp) ||
+      ((uintptr_t)a->stats & 15))
+    return S2C_EINVAL;
   const int rows = a->lg.rows;
   if (rows == 0) return 0;
   const Plan p = forward_plan(rows, a->lg.V, a->lg.dtype);
@@ -907,7 +914,7 @@ extern "C" int s2c_token_scores_fwd(const s2c_token_scores_args *a, void *stream
 
 extern "C" int s2c_token_scores_bwd(const s2c_token_scores_args *a, const float *g_logp,
                                     const float *g_entropy, const float *g_top, void *dx, void *stream) {
-  if (bad_scores(a) || !a->stats || !dx) return S2C_EINVAL;
+  if (bad_scores(a) || bad_backward(a->lg, a->stats, dx)) return S2C_EINVAL;
   if (a->lg.rows == 0) return 0;
   GradArgs g = {};
   g.lg = a->lg;
@@ -927,7 +934,7 @@ extern "C" long long s2c_distill_workspace_bytes(int rows, int V, int dtype) {
 }
 
 extern "C" int s2c_distill_fwd(const s2c_distill_args *a, void *stream) {
-  if (bad_distill(a) || !a->loss) return S2C_EINVAL;
+  if (bad_distill(a) || !a->loss || ((uintptr_t)a->stats & 15)) return S2C_EINVAL;
   const int rows = a->lg.rows;
   if (rows == 0) return 0;
   const Plan p = forward_plan(rows, a->lg.V, a->lg.dtype);
@@ -949,7 +956,7 @@ extern "C" int s2c_distill_fwd(const s2c_distill_args *a, void *stream) {
 }
 
 extern "C" int s2c_distill_bwd(const s2c_distill_args *a, const float *g_loss, void *dx, void *stream) {
-  if (bad_distill(a) || !a->stats || !g_loss || !dx) return S2C_EINVAL;
+  if (bad_distill(a) || !g_loss || bad_backward(a->lg, a->stats, dx)) return S2C_EINVAL;
   if (a->lg.rows == 0) return 0;
   GradArgs g = {};
   g.lg = a->lg;

@@ -160,8 +160,15 @@ def test_c_entries_refuse_bad_arguments():
     a = scores()
     assert lib.s2c_token_scores_fwd(None, None) == EINVAL
     assert lib.s2c_token_scores_bwd(ctypes.addressof(a), P, P, P, None, None) == EINVAL
-    a = scores(stats=None)
-    assert lib.s2c_token_scores_bwd(ctypes.addressof(a), P, P, P, P, None) == EINVAL
+    assert lib.s2c_token_scores_bwd(ctypes.addressof(a), P, P, P, P + 2, None) == EINVAL
+    for stats in (None, P + 8):
+        a = scores(stats=stats)
+        assert lib.s2c_token_scores_bwd(ctypes.addressof(a), P, P, P, P, None) == EINVAL
+    assert lib.s2c_token_scores_fwd(ctypes.addressof(a), None) == EINVAL
+    # many words of few rows: joined through a workspace
+    for ws in (None, P + 4):
+        a = scores(lg=_lg(V=1 << 18, s2=1 << 18), ws=ws)
+        assert lib.s2c_token_scores_fwd(ctypes.addressof(a), None) == EINVAL
     distill = lambda **kw: _DistillArgs(**dict(dict(    # noqa: E731
         lg=_lg(), K=3, teacher_dtype=0, ids=P, teacher=P, mask=None, loss=P, stats=P, ws=P), **kw))
     for kw in (dict(K=0), dict(K=257), dict(teacher_dtype=5), dict(ids=None), dict(teacher=None),
@@ -171,8 +178,12 @@ def test_c_entries_refuse_bad_arguments():
     d = distill()
     assert lib.s2c_distill_bwd(ctypes.addressof(d), None, P, None) == EINVAL
     assert lib.s2c_distill_bwd(ctypes.addressof(d), P, None, None) == EINVAL
-    d = distill(stats=None)
-    assert lib.s2c_distill_bwd(ctypes.addressof(d), P, P, None) == EINVAL
+    for stats in (None, P + 4):
+        d = distill(stats=stats)
+        assert lib.s2c_distill_bwd(ctypes.addressof(d), P, P, None) == EINVAL
+    assert lib.s2c_distill_fwd(ctypes.addressof(d), None) == EINVAL
+    d = distill(lg=_lg(V=1 << 18, s2=1 << 18), ws=None)
+    assert lib.s2c_distill_fwd(ctypes.addressof(d), None) == EINVAL
     fwd = lambda N=2, V=3, D=4, dt=0, ld=4, tok=P, tab=P, out=P: lib.s2c_embed_fwd(       # noqa: E731
         N, V, D, dt, ld, tok, tab, 1.0, -1, out, None)
     for kw in (dict(N=-1), dict(V=0), dict(D=0), dict(D=(1 << 24) + 1), dict(dt=3), dict(ld=-1), dict(tok=None),
@@ -183,6 +194,10 @@ def test_c_entries_refuse_bad_arguments():
     for kw in (dict(N=-1), dict(V=0), dict(D=0), dict(D=(1 << 24) + 1), dict(dt=3), dict(ld=-1), dict(tok=None),
                dict(g=None), dict(out=None), dict(g=P + 2), dict(out=P + 1, dt=2)):
         assert grad(**kw) == EINVAL, kw
+    # many tokens: sorted in a workspace
+    assert lib.s2c_embed_grad(5000, 300, 4, 0, 4, P, P, 1.0, -1, P, None, None) == EINVAL
+    assert lib.s2c_embed_grad(5000, 300, 4, 0, 4, P, P, 1.0, -1, P, P + 8, None) == EINVAL
+    assert lib.s2c_embed_grad(1 << 31, 300, 4, 0, 4, P, P, 1.0, -1, P, P, None) == EINVAL
     # nothing to do is no error and no launch
     z = scores(lg=_lg(rows=0, x=None))
     assert lib.s2c_token_scores_fwd(ctypes.addressof(z), None) == 0

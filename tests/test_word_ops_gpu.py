@@ -258,6 +258,54 @@ def test_scores_strides(V, dtype):
         _check_scores(x, _ints(x.shape[:-1], n, 16), min(5, n), T=0.9, seed=17)
 
 
+@pytest.mark.parametrize("rows,V", [(5, 200003), (300, 40000), (2500, 3501)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_every_share_of_the_rows(rows, V, dtype):
+    """Stretches of a row, a workgroup a row, a wave a row: ignored rows that hold NaN, rows of nothing,
+    rows of one value, masked rows, repeated slots and alternatives that take gradients, in each."""
+    x = _logits((rows,), V, dtype, V)
+    t = _ints((rows,), V, rows, lo=1)
+    t[1] = 0
+    x[1, ::7] = NAN
+    x[2] = -INF
+    x[3] = 1.25
+    x[4, 100:] = -INF
+    t[4] = 50
+    live = torch.ones(rows, dtype=torch.bool, device="cuda")
+    live[1] = False
+    y = x.clone()
+    y[1] = 0
+    _check_scores(y, t, 33, T=0.8, ignore=0)
+    out = word_ops.token_scores(x, t, top_k=33, temperature=0.8, ignore_index=0)
+    ref = word_ops.token_scores(y, t, top_k=33, temperature=0.8, ignore_index=0)
+    for a, b in zip(out, ref):
+        assert torch.equal(a, b)
+    ids = _ints((rows, 20), V, 5)
+    ids[:, 7] = ids[:, 3]
+    ids[3, 5:] = -1
+    w = _randn((rows, 20), 6)
+    z = torch.where(live.unsqueeze(-1), x, torch.zeros_like(x))
+    _check_distill(z, ids, w, 1.5, mask=live)
+    a = word_ops.distill_loss(x, ids, w, temperature=1.5, mask=live)
+    assert torch.equal(a, word_ops.distill_loss(z, ids, w, temperature=1.5, mask=live)) and a[1].item() == 0
+    leaf = x.clone().requires_grad_()
+    g, = torch.autograd.grad([word_ops.distill_loss(leaf, ids, w, mask=live)], [leaf], [_randn((rows,), 7)])
+    assert bool((g[1] == 0).all()) and bool((g[2] == 0).all())
+
+
+@pytest.mark.parametrize("order", ["up", "down", "same", "sawtooth"])
+@pytest.mark.parametrize("rows,V", [(2, 131073), (400, 3500), (2100, 1500)])
+def test_alternatives_of_ordered_rows(rows, V, order):
+    """Rows that fill the buffers of candidates: every element beats the last, none does, all are equal."""
+    i = torch.arange(V, device="cuda", dtype=torch.float32)
+    row = {"up": i, "down": -i, "same": i * 0, "sawtooth": i % 97}[order] / 1000
+    x = row.expand(rows, V).contiguous()
+    for k in (1, 64):
+        out = word_ops.token_scores(x, None, top_k=k)
+        want = torch.sort(row, descending=True, stable=True)[1][:k]
+        assert bool((out.top_ids == want).all())
+
+
 @pytest.mark.parametrize("shape", [(0,), (3, 0), (0, 2, 4)])
 def test_empty_batches(shape):
     x = torch.empty(shape + (9,), device="cuda", requires_grad=True)
