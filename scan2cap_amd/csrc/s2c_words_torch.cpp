@@ -65,9 +65,14 @@ void check_gpu(const char *name, const Tensor &t, const Tensor &like) {
   check_place(t.device() == like.device(), name, " is on ", t.device(), ", the other tensors on ", like.device());
 }
 
-Tensor ids64(const Tensor &t) { return t.to(at::kLong).contiguous(); }
+// (the usual case costs no dispatch)
+Tensor dense(const Tensor &t, at::ScalarType type) {
+  return t.scalar_type() == type && t.is_contiguous() ? t : t.to(type).contiguous();
+}
 
-Tensor f32(const Tensor &g) { return g.to(at::kFloat).contiguous(); }
+Tensor ids64(const Tensor &t) { return dense(t, at::kLong); }
+
+Tensor f32(const Tensor &g) { return dense(g, at::kFloat); }
 
 // a tensor's data, NULL for an undefined one
 template <class T>

@@ -43,10 +43,11 @@ def _load():
 _ext = _load()
 
 
-def _check_tensors(**tensors):
+def _refuse(**tensors):
+    """After a TypeError of the binding: say which argument is no tensor."""
     for name, t in tensors.items():
         if not torch.is_tensor(t):
-            raise ValueError("%s must be a tensor, not %s" % (name, type(t).__name__))
+            raise ValueError("%s must be a tensor, not %s" % (name, type(t).__name__)) from None
 
 
 def token_scores(logits, tokens=None, top_k=0, temperature=1.0, ignore_index=None):
@@ -64,8 +65,11 @@ def token_scores(logits, tokens=None, top_k=0, temperature=1.0, ignore_index=Non
     = -1 (an empty slot of `distill_loss`), zero gradient.  Logits of -inf are words that cannot be said;
     a row of nothing else has logp -inf, entropy 0 and zero gradient.  A token outside [0, V) makes logp
     and the row's gradient NaN, as a logit of NaN or +inf does to everything in its row."""
-    _check_tensors(logits=logits)
-    return TokenScores(*_ext.token_scores(logits, tokens, top_k, temperature, ignore_index))
+    try:
+        return TokenScores._make(_ext.token_scores(logits, tokens, top_k, temperature, ignore_index))
+    except TypeError:
+        _refuse(logits=logits)
+        raise
 
 
 def distill_loss(logits, teacher_ids, teacher_logits, temperature=1.0, mask=None):
@@ -79,8 +83,11 @@ def distill_loss(logits, teacher_ids, teacher_logits, temperature=1.0, mask=None
     mask (..., bool) False are not read; they and rows without a used slot have loss 0 and zero gradient.
     A used id >= V makes the row's loss and gradient NaN; a row of logits that are all -inf has loss +inf
     and zero gradient."""
-    _check_tensors(logits=logits, teacher_ids=teacher_ids, teacher_logits=teacher_logits)
-    return _ext.distill_loss(logits, teacher_ids, teacher_logits, temperature, mask)
+    try:
+        return _ext.distill_loss(logits, teacher_ids, teacher_logits, temperature, mask)
+    except TypeError:
+        _refuse(logits=logits, teacher_ids=teacher_ids, teacher_logits=teacher_logits)
+        raise
 
 
 def embed_tokens(tokens, table, scale=1.0, padding_idx=None):
@@ -88,5 +95,8 @@ def embed_tokens(tokens, table, scale=1.0, padding_idx=None):
     strided) -> (..., D) of the table's type.  Tokens equal to `padding_idx` (any integer) give zeros and
     no gradient; a token outside [0, V) gives a row of NaN and no gradient.  The table's gradient is
     dense, summed in float32 over each word's places in their order (the same bits every time)."""
-    _check_tensors(tokens=tokens, table=table)
-    return _ext.embed_tokens(tokens, table, scale, padding_idx)
+    try:
+        return _ext.embed_tokens(tokens, table, scale, padding_idx)
+    except TypeError:
+        _refuse(tokens=tokens, table=table)
+        raise
