@@ -18,8 +18,12 @@
 // to its k best, by counting ranks; later elements equal to a wave's own k-th have lost, since a wave
 // walks its tiles in index order.
 //
-// All of it is bound by reading the logits (and, backward, reading them again and writing the
-// gradient).
+// All of it is bound by reading the logits and, backward, reading them again and writing the gradient; a
+// copy of 1 GiB reaches 5.1 TB/s here.  Kernel times on MI355X: 59392 x 3500 fp32 with 5 alternatives 161 us
+// (5.2 TB/s); 4096 x 50001 bf16 with 8 alternatives, a tenth of the rows ignored, 92 us forward (4.0 TB/s:
+// about half of it is the VALU's, 8 instructions an element) and 126 us backward; distillation over
+// 4096 x 65536 bf16 with 64 slots 115 us and 180 us (6.0 TB/s); one row of 32768 bf16 words 8 us (a launch, a
+// trip to memory and the selection's chain of ballots).
 #include "s2c_words_common.h"
 
 #include <stdio.h>
@@ -97,7 +101,10 @@ struct Best {
 #pragma unroll
     for (int i = 0; i < 3; ++i) e[i] = lane + 64 * i < cnt ? buf[lane + 64 * i] : 0;
     if (cnt <= 64) {            // the common case stays in registers
-      for (int j = 0; j < cnt; ++j) rank[0] += readlane_u64(e[0], j) > e[0];
+      for (int j = 0; j < cnt; j += 4) {                        // (lanes from cnt on hold 0)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) rank[0] += readlane_u64(e[0], j + q) > e[0];
+      }
     } else {
       for (int j = 0; j < cnt; ++j) {
         const u64 o = buf[j];
@@ -222,7 +229,29 @@ __device__ __forceinline__ void stream_tile(const char *xr, int V, int shift, in
       best.bound = kth_of_lanes(key, best.k);
     }
     const float thr = best.threshold();
-    if (__ballot(!(tmax <= thr))) {
+    const bool enter = __ballot(!(tmax <= thr)) != 0;
+    if (enter && G > 1) {
+      // few rows: what passes is rare and the code's length counts -- a mask of every lane's elements, then
+      // one of each lane at a time, read again (512 rows of 32000 words, 8 alternatives: 13.7 us, 14.7 with the
+      // elements unrolled as below).  A wave of its own per row meets more of them (59392 rows of 3500, 5
+      // alternatives: 161 us unrolled, 263 us when masks were tried there).
+      u32 hits = 0;
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) hits |= (!(E::at(r[u], e) <= thr) ? 1u : 0u) << (u * VEC + e);
+      while (__ballot(hits != 0)) {
+        const int b = __builtin_ctz(hits | 0x80000000u);
+        const int vi = t0 + (b / VEC) * 64 + lane;
+        const u32 idx = (u32)vi * VEC - shift + (b & (VEC - 1));     // (negative: above V)
+        const bool ok = hits != 0 && vi < ve && idx < (u32)V;
+        const u64 key = ((u64)ord(ok ? E::load(xr, idx) : 0.0f) << 32) | (u32)~idx;
+        const u64 mask = __ballot(ok && key > best.kth);
+        hits &= hits - 1;
+        if (mask) best.add(mask, key, lane);
+      }
+    }
+    if (enter && G == 1) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         if (!INSIDE && u >= nu) break;
