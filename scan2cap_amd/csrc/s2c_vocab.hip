@@ -47,8 +47,24 @@ __device__ __forceinline__ float nan_max(float a, float b) { return __builtin_el
 constexpr float D_MIN = -160.0f;
 
 __device__ __forceinline__ const char *row_ptr(const s2c_logits &lg, int es, int r) {
+  if (lg.n2 == lg.rows) return (const char *)lg.x + es * (r * lg.s2);      // (no divisions for rows of one stride)
   const int i2 = r % lg.n2, t = r / lg.n2, i1 = t % lg.n1, i0 = t / lg.n1;
   return (const char *)lg.x + es * (i0 * lg.s0 + i1 * lg.s1 + i2 * lg.s2);
+}
+
+// a wave's number in its workgroup, in a scalar register: what follows from it (rows, addresses, conditions)
+// is then computed once for the wave
+__device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); }
+
+// unit `un` = (row, stretch) of rows in `n` stretches
+__device__ __forceinline__ void row_and_stretch(long long un, int n, int &r, int &seg) {
+  if (n == 1) {
+    r = (int)un;
+    seg = 0;
+  } else {
+    r = (int)(un / n);
+    seg = (int)(un - (long long)r * n);
+  }
 }
 
 // ---- order-preserving keys ---------------------------------------------------------------------------
@@ -341,7 +357,7 @@ template <int DT, int G, bool TOP, bool ENT>
 __device__ __forceinline__ Stat group_stat(const char *xr, int V, int seg, int segs, int k, float c,
                                            u64 (*lists)[BUF], Stat *s_part, Shared *sh) {
   typedef Elem<DT> E;
-  const int lane = lane_id(), w = G == 1 ? 0 : (int)(threadIdx.x >> 6);
+  const int lane = lane_id(), w = G == 1 ? 0 : wave_id();
   const int shift = (int)(((uintptr_t)xr / E::ES) & (E::VEC - 1));
   const int nvec = (int)(((long long)V + shift + E::VEC - 1) / E::VEC);
   const int per = (nvec + segs - 1) / segs;
@@ -459,7 +475,7 @@ __global__ __launch_bounds__(Shape<G>::THREADS) void scores_fwd_kernel(s2c_token
   __shared__ u64 s_lists[TOP ? Sh::WAVES + (G > 1) : 1][TOP ? BUF : 1];
   __shared__ Stat s_part[Sh::WAVES];
   __shared__ Shared s_shared;
-  const int lane = lane_id(), w = threadIdx.x >> 6;
+  const int lane = lane_id(), w = wave_id();
   const int grp = G == 1 ? w : 0;
   const bool first = G == 1 || w == 0;
   if (TOP && G > 1) {
@@ -470,7 +486,8 @@ __global__ __launch_bounds__(Shape<G>::THREADS) void scores_fwd_kernel(s2c_token
   const float c = a.lg.inv_t * LOG2E;
   const long long units = (long long)a.lg.rows * sp.n;
   for (long long un = (long long)blockIdx.x * Sh::GROUPS + grp; un < units; un += (long long)gridDim.x * Sh::GROUPS) {
-    const int r = (int)(un / sp.n), seg = (int)(un % sp.n);
+    int r, seg;
+    row_and_stretch(un, sp.n, r, seg);
     if (scores_dead(a, r)) {
       if (first && sp.n == 1) scores_write_dead(a, r, lane);
       continue;
@@ -489,7 +506,7 @@ __global__ __launch_bounds__(Shape<G>::THREADS) void scores_fwd_kernel(s2c_token
 template <int DT>
 __global__ __launch_bounds__(256) void scores_join_kernel(s2c_token_scores_args a, Split sp) {
   __shared__ u64 s_list[4][BUF];
-  const int lane = lane_id(), w = threadIdx.x >> 6;
+  const int lane = lane_id(), w = wave_id();
   const float c = a.lg.inv_t * LOG2E;
   for (long long r = (long long)blockIdx.x * 4 + w; r < a.lg.rows; r += (long long)gridDim.x * 4) {
     if (scores_dead(a, (int)r)) {
@@ -579,13 +596,14 @@ template <int DT, int G>
 __global__ __launch_bounds__(Shape<G>::THREADS) void distill_fwd_kernel(s2c_distill_args a, Split sp) {
   typedef Shape<G> Sh;
   __shared__ Stat s_part[Sh::WAVES];
-  const int lane = lane_id(), w = threadIdx.x >> 6;
+  const int lane = lane_id(), w = wave_id();
   const int grp = G == 1 ? w : 0;
   const bool first = G == 1 || w == 0;
   const float c = a.lg.inv_t * LOG2E;
   const long long units = (long long)a.lg.rows * sp.n;
   for (long long un = (long long)blockIdx.x * Sh::GROUPS + grp; un < units; un += (long long)gridDim.x * Sh::GROUPS) {
-    const int r = (int)(un / sp.n), seg = (int)(un % sp.n);
+    int r, seg;
+    row_and_stretch(un, sp.n, r, seg);
     bool dead = a.mask && a.mask[r] == 0;
     const char *xr = row_ptr(a.lg, Elem<DT>::ES, r);
     Slots t;
@@ -610,7 +628,7 @@ __global__ __launch_bounds__(Shape<G>::THREADS) void distill_fwd_kernel(s2c_dist
 
 template <int DT>
 __global__ __launch_bounds__(256) void distill_join_kernel(s2c_distill_args a, Split sp) {
-  const int lane = lane_id(), w = threadIdx.x >> 6;
+  const int lane = lane_id(), w = wave_id();
   const float c = a.lg.inv_t * LOG2E;
   for (long long r = (long long)blockIdx.x * 4 + w; r < a.lg.rows; r += (long long)gridDim.x * 4) {
     bool dead = a.mask && a.mask[r] == 0;
@@ -673,13 +691,14 @@ __global__ __launch_bounds__(256) void vocab_bwd_kernel(GradArgs a) {
   };
   __shared__ Entries s_entries[GROUPS];
   const int lane = lane_id();
-  const int grp = G == 1 ? (int)(threadIdx.x >> 6) : 0, tid = G == 1 ? lane : (int)threadIdx.x;
+  const int grp = G == 1 ? wave_id() : 0, tid = G == 1 ? lane : (int)threadIdx.x;
   Entries &en = s_entries[grp];
   const float c = a.lg.inv_t * LOG2E, it = a.lg.inv_t;
   const int V = a.lg.V;
   const long long units = (long long)a.lg.rows * a.segs;
   for (long long un = (long long)blockIdx.x * GROUPS + grp; un < units; un += (long long)gridDim.x * GROUPS) {
-    const int r = (int)(un / a.segs), seg = (int)(un % a.segs);
+    int r, seg;
+    row_and_stretch(un, a.segs, r, seg);
     const char *xr = row_ptr(a.lg, E::ES, r);
     const long long o0 = (long long)r * V;
     const int shift = (int)((((uintptr_t)a.dx / E::ES) + o0) & (VEC - 1));       // of the stores

@@ -486,7 +486,8 @@ def _check_embed(tokens, table, scale=1.0, pad=None, g=None, seed=0):
 @pytest.mark.parametrize("N,V,D", [(1, 1, 1), (1, 5, 3), (7, 3, 8), (65, 10, 300), (256, 3500, 300), (1000, 97, 515),
                                    (2048, 64, 64), (2049, 64, 64), (4096, 3500, 33), (8191, 1001, 40),
                                    (8193, 513, 24), (20000, 70000, 16), (70001, 257, 9), (300, 5, 4099),
-                                   (100000, 1, 8), (9000, 131072, 4)])
+                                   (100000, 1, 8), (9000, 131072, 4), (700001, 1000, 3), (3000017, 70000, 2),
+                                   (600, 3, 1 << 20), (512, 131072, 2), (513, 131071, 2), (400, 300000, 1)])
 def test_embed_over_sizes(N, V, D, dtype):
     _check_embed(_ints((N,), V, N), _logits((V,), D, dtype, V, 1.0), scale=1.7, seed=D)
 
