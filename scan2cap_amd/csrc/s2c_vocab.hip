@@ -852,7 +852,8 @@ long long vectors(int V, int dtype) {                  // of a row, at any align
 
 // How a row is shared out: `waves` of a workgroup to a stretch, `split` stretches to a row.
 //  * many rows: a wave each -- no barrier, no merge, one threshold for the whole row (59392 rows of 3500
-//    fp32 words, 5 alternatives: 161 us, against 292 us with 4 waves a row);
+//    fp32 words, 5 alternatives: 161 us, against 292 us with 4 waves a row; 150 us since its row lives in
+//    scalar registers);
 //  * rows that would leave most of the chip empty: 16 waves (32768 bf16 words, one row: 8.0 us, 9.7 with 4,
 //    20.9 with 1), and stretches of at least one round of tiles, up to 256 workgroups, joined by a second
 //    launch (64 rows of 131072 words: 17.4 us in 4 stretches, 18.6 in one; one row of 262144 fp32 words: 14.2
@@ -894,7 +895,11 @@ Split split_of(const Plan &p, int rows, int k, void *ws) {
 template <bool DISTILL>
 int backward(GradArgs &a, const char *what, hipStream_t st) {
   const long long nvec = vectors(a.lg.V, a.lg.dtype);
-  const int G = nvec <= 64 * U ? 1 : 4;
+  // waves of their own for short rows, whose stretches would leave most of a workgroup idle (59392 x 3500 bf16,
+  // 439 vectors: 154 us, 277 with 4 waves; 8192 x 8000, 1001 vectors: 48.5 and 45 us), and further where a
+  // stretch waits for its slots (the same with 32 slots: 52 and 56 us; 1000 x 10007, 33 slots: 13.4 and 17.7;
+  // 4096 x 65536, 64 slots: 206 and 182)
+  const int G = nvec <= (DISTILL ? 2048 : 512) ? 1 : 4;
   a.segs = (int)((nvec + 64 * G * U - 1) / (64 * G * U));
   a.span = (int)((nvec + a.segs - 1) / a.segs);
   // a gradient that the 256 MB cache cannot hold would leave it full of lines to be written back: the

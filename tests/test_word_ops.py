@@ -7,6 +7,7 @@ import re
 import pytest
 import torch
 
+from tests import words_common  # noqa: F401  (first: the binding)
 from scan2cap_amd import _C, word_ops
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))

@@ -12,6 +12,7 @@ import math
 import pytest
 import torch
 
+from tests import words_common  # noqa: F401  (first: the binding)
 from scan2cap_amd import word_ops
 
 pytestmark = pytest.mark.gpu

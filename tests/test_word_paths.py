@@ -7,6 +7,7 @@ import torch
 
 from tests import golden_common as gc
 from tests import plain_caption_common as pc
+from tests import words_common  # noqa: F401  (first: the binding)
 
 DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
 U = 2.0 ** -24
