@@ -19,6 +19,7 @@ extern "C" {
 #define S2C_WORDS_MAX_TOP 64     /* alternatives of s2c_token_scores */
 #define S2C_WORDS_MAX_SLOTS 256  /* teacher words per row of s2c_distill */
 #define S2C_WORDS_MAX_DIM (1 << 24) /* columns of an embedding table */
+#define S2C_WORDS_NO_PADDING (-9223372036854775807LL - 1) /* `padding` where no token is padding */
 
 /* Word logits: `rows` rows of V elements (unit stride inside a row) of type `dtype`; row r starts at
  *   x + (r / (n1 n2)) s0 + (r / n2 % n1) s1 + (r % n2) s2        (elements)
@@ -84,7 +85,8 @@ int s2c_distill_bwd(const s2c_distill_args *a, const float *g_loss, void *dx, vo
 long long s2c_words_args_sizeof(int which);
 
 /* out (N, D) contiguous = scale * table[token] (table (V, D): unit column stride, row stride `ld`
- * elements); a token equal to `padding` gives zeros, one outside [0, V) a row of NaN. */
+ * elements); a token equal to `padding` (unless that is S2C_WORDS_NO_PADDING) gives zeros, any other one
+ * outside [0, V) a row of NaN. */
 int s2c_embed_fwd(long long N, int V, int D, int dtype, long long ld, const long long *token,
                   const void *table, float scale, long long padding, void *out, void *stream);
 /* d_table (V, D) contiguous, every row written: scale * sum of g (N rows, row stride ldg) over the

@@ -76,10 +76,11 @@ __global__ __launch_bounds__(THREADS) void embed_fwd_kernel(long long N, int V, 
       for (int i = 0; i < ROWS; ++i) {
         const long long n = n0 + i * per;
         if (n >= N) break;
-        const bool bad = t[i] != padding && (t[i] < 0 || t[i] >= V);
+        const bool pad = t[i] == padding && padding != S2C_WORDS_NO_PADDING;
+        const bool bad = !pad && (t[i] < 0 || t[i] >= V);
         float f[E::VEC];
 #pragma unroll
-        for (int e = 0; e < E::VEC; ++e) f[e] = bad ? NAN : t[i] == padding ? 0.0f : scale * E::at(r[i], e);
+        for (int e = 0; e < E::VEC; ++e) f[e] = bad ? NAN : pad ? 0.0f : scale * E::at(r[i], e);
         if (past_cache) store16_past_cache(out, (n * D + c) * E::ES, E::pack(f));
         else store_part<DT>(out, n * D + c, D - c, f);
       }

@@ -156,7 +156,10 @@ Tensor first_order(const Tensor &g) {
   return (*error)({v})[0];
 }
 
-bool wants_grad(const Tensor &t) { return at::GradMode::is_enabled() && t.requires_grad(); }
+// (a forward-mode tangent goes through the autograd node too, which refuses it)
+bool wants_grad(const Tensor &t) {
+  return (at::GradMode::is_enabled() && t.requires_grad()) || t._fw_grad(/*level=*/0).defined();
+}
 
 // ---- token_scores ----------------------------------------------------------------------------------------------
 struct Scores { Tensor logp, entropy, top_logp, top_ids, stats; };
@@ -362,8 +365,6 @@ Tensor distill_loss(const Tensor &logits, const Tensor &ids, const Tensor &teach
 }
 
 // ---- embed_tokens ----------------------------------------------------------------------------------------------
-constexpr long long NO_WORD = -(1LL << 62) - (1LL << 62);          // no padding word
-
 Tensor embed_forward(const Tensor &tokens, const Tensor &table, double scale, int64_t padding) {
   const c10::DeviceGuard guard(table.device());
   std::vector<int64_t> shape = tokens.sizes().vec();
@@ -425,7 +426,8 @@ Tensor embed_tokens(const Tensor &tokens, const Tensor &table, double scale, std
   check_gpu("table", table, table);
   check_gpu("tokens", tokens, table);
   const Tensor t = ids64(tokens);
-  const int64_t pad = padding.value_or(NO_WORD);
+  check(padding != std::optional<int64_t>(S2C_WORDS_NO_PADDING), "padding_idx cannot be the lowest integer");
+  const int64_t pad = padding.value_or(S2C_WORDS_NO_PADDING);
   return wants_grad(table) ? EmbedFn::apply(t, table, scale, pad) : embed_forward(t, table, scale, pad);
 }
 

@@ -12,6 +12,10 @@ nothing synchronises, scratch memory is allocated per call.  Arguments that the 
 refused with ValueError (shapes, types, ranges) or RuntimeError (CPU tensors: there is no fallback).
 Values that live on the device cannot be refused without a synchronisation: a word index outside the
 vocabulary is never used as an address and turns its row's results into NaN.
+
+Everything may be captured into a graph and replayed.  A backward pass is captured while no eager graph of
+the same leaves is alive (drop its outputs first): torch would synchronise the leaves' own stream inside
+the capture, which it does not survive.  Second derivatives and forward-mode tangents are refused.
 """
 import collections
 import importlib.machinery
@@ -92,9 +96,10 @@ def distill_loss(logits, teacher_ids, teacher_logits, temperature=1.0, mask=None
 
 def embed_tokens(tokens, table, scale=1.0, padding_idx=None):
     """scale * table[tokens]: tokens (...) int64 or int32, table (V, D) with adjacent columns (rows may be
-    strided) -> (..., D) of the table's type.  Tokens equal to `padding_idx` (any integer) give zeros and
-    no gradient; a token outside [0, V) gives a row of NaN and no gradient.  The table's gradient is
-    dense, summed in float32 over each word's places in their order (the same bits every time)."""
+    strided) -> (..., D) of the table's type.  Tokens equal to `padding_idx` (any integer but int64's lowest,
+    in the table or not) give zeros and no gradient; a token outside [0, V) gives a row of NaN and no
+    gradient.  The table's gradient is dense, summed in float32 over each word's places in their order (the
+    same bits every time)."""
     try:
         return _ext.embed_tokens(tokens, table, scale, padding_idx)
     except TypeError:

@@ -505,6 +505,15 @@ def test_embed_padding_and_bad_tokens(N):
     _check_embed(torch.full((N,), 7, device="cuda"), table, 2.0)                 # one word
 
 
+def test_embed_lowest_token_is_a_bad_one():
+    t = torch.tensor([3, -2 ** 63, 2 ** 63 - 1, 0, -1], device="cuda")
+    table = _logits((5,), 20, torch.float32, 42, 1.0)
+    for pad in (None, 0, 2 ** 63 - 1):
+        _check_embed(t, table, 0.5, pad)
+    with pytest.raises(ValueError):
+        word_ops.embed_tokens(t, table, padding_idx=-2 ** 63)
+
+
 def test_embed_one_word_takes_most_places():
     t = _ints((40000,), 300, 43)
     t[_ints((30000,), 40000, 44)] = 2
@@ -597,6 +606,21 @@ def test_second_derivatives_are_refused():
         assert bool(g.isfinite().all())
         with pytest.raises(RuntimeError, match="once_differentiable"):
             g.sum().backward()
+
+
+def test_forward_mode_tangents_are_refused():
+    import torch.autograd.forward_ad as fwAD
+    x, table = _logits((3,), 50, torch.float32, 62), _logits((50,), 4, torch.float32, 63)
+    t, ids = _ints((3,), 50, 64), _ints((3, 2), 50, 65)
+    w = torch.zeros(3, 2, device="cuda")
+    with fwAD.dual_level():
+        dx, dtable, dw = (fwAD.make_dual(v, torch.ones_like(v)) for v in (x, table, w))
+        for call in (lambda: word_ops.token_scores(dx, t), lambda: word_ops.distill_loss(dx, ids, w),
+                     lambda: word_ops.embed_tokens(t, dtable)):
+            with pytest.raises(RuntimeError, match="jvp"):
+                call()
+        with pytest.raises(ValueError, match="detach"):
+            word_ops.distill_loss(x, ids, dw)
 
 
 def test_on_another_stream():
