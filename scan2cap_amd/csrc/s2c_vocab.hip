@@ -19,11 +19,11 @@
 // walks its tiles in index order.
 //
 // All of it is bound by reading the logits and, backward, reading them again and writing the gradient; a
-// copy of 1 GiB reaches 5.1 TB/s here.  Kernel times on MI355X: 59392 x 3500 fp32 with 5 alternatives 161 us
-// (5.2 TB/s); 4096 x 50001 bf16 with 8 alternatives, a tenth of the rows ignored, 92 us forward (4.0 TB/s:
-// about half of it is the VALU's, 8 instructions an element) and 126 us backward; distillation over
-// 4096 x 65536 bf16 with 64 slots 115 us and 180 us (6.0 TB/s); one row of 32768 bf16 words 8 us (a launch, a
-// trip to memory and the selection's chain of ballots).
+// copy of 1 GiB reaches 5.1 TB/s here.  Kernel times on MI355X: 59392 x 3500 fp32 with 5 alternatives 157 us
+// (5.3 TB/s); 4096 x 50001 bf16 with 8 alternatives, a tenth of the rows ignored, 85 us forward (4.3 TB/s:
+// about half of it is the VALU's, 8 instructions an element) and 128 us backward; distillation over
+// 4096 x 65536 bf16 with 64 slots 116 us and 183 us (5.9 TB/s); one row of 32768 bf16 words 7.4 us (a launch,
+// a trip to memory and the selection's chain of ballots).
 #include "s2c_words_common.h"
 
 #include <stdio.h>
