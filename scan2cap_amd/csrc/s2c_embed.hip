@@ -10,11 +10,12 @@
 //  * a stable sort of (word, place) by word; padding and bad tokens sort behind the last word.  The sorted
 //    order is cut into chunks, a wave each, whatever words are in them (a word's run may be most of the
 //    batch, or one place): the wave has 4 to 8 of its rows under way and writes a word's sum when its run ends.
-//    A run that passes a chunk's border leaves partial sums, which a last launch joins in order; it also
-//    writes the rows of the words that are not in the batch.
-// Measured (kernel times, MI355X): 131072 tokens x 1024 bf16, 50001 words: lookup 79 us (4.1 TB/s),
-// gradient 135 us = sort 31 + runs 79 + join 25 (floor 73 us at 5.1 TB/s); 8191 x 515 fp16, 10007 words:
-// lookup 5.6 us, gradient 35 us = sort 18 + 9 + 8.
+//    A run that passes a chunk's border leaves partial sums, which a last launch joins in order, 16 waves to a
+//    long run (10^6 x 256 bf16 whose most frequent word takes 4 %: 30 us, 73 with 4).  The rows of the
+//    words that are not in the batch are written beside the sums.
+// Measured (kernel times, MI355X): 131072 tokens x 1024 bf16, 50001 words: lookup 80 us (4.1 TB/s),
+// gradient 120 us = sort 28 + runs 82 + join 10 (floor 73 us at 5.1 TB/s); 8191 x 515 fp16, 10007 words:
+// lookup 5.7 us, gradient 35 us = sort 18 + 10 + 7.
 #include "s2c_words_common.h"
 
 #include <stdio.h>
@@ -118,7 +119,7 @@ struct GradArgs {
   const void *g;
   void *dt;
   // the sorted order
-  u32 *key, *pos, *start;        // (N), (N), (V + 1)
+  u32 *key, *pos;                // (N) each
   int chunk;                     // places of it that a wave takes, <= 64
   float *partial;                // (chunks, 2, ldp): a chunk's run that began before it, one that goes on
   int ldp;                       // D, up to a multiple of 8
@@ -311,7 +312,7 @@ __global__ __launch_bounds__(THREADS) void sort_scatter_kernel(SortArgs a) {
   {
     // this workgroup's first place of digit tid: all smaller digits, then the workgroups before it
     u32 total = 0, before = 0;
-#pragma unroll 8
+#pragma unroll 32
     for (u32 i = 0; i < gridDim.x; ++i) {
       const u32 x = a.counts[(size_t)i * RADIX + tid];
       total += x;
@@ -364,21 +365,75 @@ __global__ __launch_bounds__(THREADS) void sort_scatter_kernel(SortArgs a) {
 
 constexpr int BATCH = 4;          // rows of a chunk that are asked for together
 
-// The first `sums` workgroups: the sums of the chunks' runs.  The others: start[v], the first place of word v
-// in the sorted order.
+constexpr int WORDS = 32, GROUP = 8;      // of a workgroup that looks for absent words: words, pieces of their columns
+
+// which of the WORDS words from v0 are in the batch (a bit each).  A trip to memory takes about 0.7 us, so
+// the places of the words' keys are narrowed 64 fold a trip, and few keys are all read at once.
+__device__ __forceinline__ u64 present_words(const GradArgs &a, u32 v0, int lane) {
+  const u32 v[2] = {v0, v0 + WORDS}, end = (u32)a.N;
+  u32 at[2] = {0u, 0u};                              // the first key that is not below v[t]: at .. at + span
+  for (u32 span = end; span;) {
+    const u32 step = (span + 63) / 64, last = (lane + 1) * step - 1;
+    u32 key[2];                                      // (no condition on a load: they go together)
+#pragma unroll
+    for (int t = 0; t < 2; ++t) key[t] = a.key[min(at[t] + last, end - 1)];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) at[t] += __popcll(__ballot(at[t] + last < end && key[t] < v[t])) * step;
+    span = step - 1;
+  }
+  u64 present = 0;
+  if (at[1] - at[0] <= 8 * 64) {
+    u32 key[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const u32 j = at[0] + i * 64 + lane;
+      const u32 k = a.key[min(j, end - 1u)];
+      key[i] = j < at[1] ? k : 0xFFFFFFFFu;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (key[i] != 0xFFFFFFFFu) present |= 1ull << (key[i] - v0);
+    for (int k = 1; k < 64; k <<= 1) present |= __shfl_xor(present, k);
+    return present;
+  }
+  u32 lo = at[0], hi = at[1];
+  while (lo < hi) {
+    const u32 mid = lo + (hi - lo) / 2;
+    if (a.key[mid] < v0 + lane) lo = mid + 1; else hi = mid;
+  }
+  return __ballot(lo < at[1] && a.key[lo < at[1] ? lo : at[0]] == v0 + lane);
+}
+
+// The rows of the words that are not in the batch.  A wave writes few of them, one after the other: 64 words to
+// a workgroup take longer where the table is small (3500 rows of 8 KB: runs 24 us, 22 with 32), 8 where it is
+// large (131072 rows of 1 KB: 36 us, 22).
+template <int DT>
+__device__ __forceinline__ void absent_rows(const GradArgs &a, long long first, long long step) {
+  const int lane = lane_id(), w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const int groups = (a.pieces + GROUP - 1) / GROUP;
+  const long long units = ((long long)a.V + WORDS - 1) / WORDS * groups;
+  for (long long un = first; un < units; un += step) {
+    const long long part = groups == 1 ? un : un / groups;
+    const int v0 = (int)(part * WORDS), p0 = (int)(un - part * groups) * GROUP, p1 = min(a.pieces, p0 + GROUP);
+    u64 absent = ~present_words(a, (u32)v0, lane);
+    absent &= __ballot(lane < WORDS && lane < a.V - v0 && (lane & (WAVES - 1)) == w);
+    for (; absent; absent &= absent - 1) {
+      const long long row = (long long)(v0 + __builtin_ctzll(absent)) * a.D;
+      for (int p = p0; p < p1; ++p) {
+        Acc<DT> zero;
+        zero.clear();
+        zero.store(a.dt, row, (p * 64 + lane) * Elem<DT>::VEC, a.D, 1.0f);
+      }
+    }
+  }
+}
+
+// The first `sums` workgroups: the sums of the chunks' runs.  The others: the rows of the absent words.
 template <int DT>
 __global__ __launch_bounds__(THREADS) void embed_runs_kernel(GradArgs a, int sums) {
   typedef Elem<DT> E;
   if ((int)blockIdx.x >= sums) {
-    const long long step = (long long)(gridDim.x - sums) * THREADS;
-    for (long long v = (long long)(blockIdx.x - sums) * THREADS + threadIdx.x; v <= a.V; v += step) {
-      u32 lo = 0, hi = (u32)a.N;
-      while (lo < hi) {
-        const u32 mid = lo + (hi - lo) / 2;
-        if (a.key[mid] < (u32)v) lo = mid + 1; else hi = mid;
-      }
-      a.start[v] = lo;
-    }
+    absent_rows<DT>(a, (long long)blockIdx.x - sums, (long long)gridDim.x - sums);
     return;
   }
   const int lane = lane_id(), w = threadIdx.x >> 6;
@@ -452,29 +507,43 @@ __device__ __forceinline__ void add_partials(Acc<DT> &acc, const GradArgs &a, u3
   }
 }
 
-constexpr u32 LONG = 16;          // chunks of a run that the four waves of a workgroup join together
+constexpr int JOIN_WAVES = 16;
+constexpr u32 LONG = 16;          // chunks of a run that the waves of a workgroup join together, more than
 
-// a workgroup: WAVES words, one piece of their columns; words far apart, since frequent ones tend to be
-// neighbours
+// the chunks [c, end) of the run that begins in chunk c and passes its end; end = c: none does
+__device__ __forceinline__ u32 run_end(const GradArgs &a, long long c, u32 &word) {
+  const long long i0 = c * a.chunk, i1 = i0 + a.chunk;
+  if (i1 >= a.N) return (u32)c;
+  // the next 64 chunks at once: most runs end there (no condition on a load: all go together)
+  const long long j = (c + 1 + lane_id()) * a.chunk;
+  const u32 next = a.key[i1], before = a.key[max(i0, 1LL) - 1], begin = a.key[min(j, a.N - 1)];
+  word = a.key[i1 - 1];
+  if (word >= (u32)a.V || next != word || (i0 > 0 && before == word)) return (u32)c;
+  const u64 more = __ballot(j < a.N && begin == word);
+  if (~more) return (u32)(c + 1 + __builtin_ctzll(~more));
+  long long lo = c + 65, hi = (a.N + a.chunk - 1) / a.chunk;       // the first chunk that begins otherwise
+  while (lo < hi) {
+    const long long mid = (lo + hi) / 2;
+    if (a.key[mid * a.chunk] == word) lo = mid + 1; else hi = mid;
+  }
+  return (u32)lo;
+}
+
+// a workgroup: the runs that begin in JOIN_WAVES chunks and pass their ends, one piece of their columns; chunks far
+// apart, since the words of long runs may be neighbours
 template <int DT>
-__global__ __launch_bounds__(THREADS) void embed_join_kernel(GradArgs a) {
+__global__ __launch_bounds__(64 * JOIN_WAVES) void embed_join_kernel(GradArgs a) {
   typedef Elem<DT> E;
-  __shared__ u32 s_c0[WAVES], s_c1[WAVES];                        // the words with a long run
-  __shared__ float s_sum[WAVES][E::VEC][64];
-  const int lane = lane_id(), w = threadIdx.x >> 6;
-  const long long quarter = ((long long)a.V + WAVES - 1) / WAVES, units = quarter * a.pieces;
+  __shared__ u32 s_c0[JOIN_WAVES], s_c1[JOIN_WAVES];                        // the long runs
+  __shared__ float s_sum[JOIN_WAVES][E::VEC][64];
+  const int lane = lane_id(), w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+  const long long chunks = (a.N + a.chunk - 1) / a.chunk;
+  const long long per = (chunks + JOIN_WAVES - 1) / JOIN_WAVES, units = per * a.pieces;
   for (long long un = blockIdx.x; un < units; un += gridDim.x) {
-    const long long v = w * quarter + un / a.pieces;
+    const u32 c0 = (u32)(w * per + un / a.pieces);
     const int col = ((int)(un % a.pieces) * 64 + lane) * E::VEC;
-    u32 s = 0, e = 0, c0 = 0, c1 = 0;
-    if (v < a.V) {
-      s = a.start[v];
-      e = a.start[v + 1];
-      if (e > s) {
-        c0 = s / a.chunk;
-        c1 = (e - 1) / a.chunk + 1;
-      }
-    }
+    u32 word = 0;
+    const u32 c1 = run_end(a, c0, word);
     const bool many = c1 - c0 > LONG;
     if (lane == 0) {
       s_c0[w] = many ? c0 : 0;
@@ -482,16 +551,16 @@ __global__ __launch_bounds__(THREADS) void embed_join_kernel(GradArgs a) {
     }
     Acc<DT> acc;
     acc.clear();
-    if (v < a.V && !many && c1 - c0 != 1) {                       // absent, or over a few chunks
+    if (c1 > c0 && !many) {
       add_partials<DT>(acc, a, c0, c0, c1, col);
-      acc.store(a.dt, v * a.D, col, a.D, a.scale);
+      acc.store(a.dt, (long long)word * a.D, col, a.D, a.scale);
     }
     __syncthreads();
-    for (int i = 0; i < WAVES; ++i) {
+    for (u64 runs = __ballot(lane < JOIN_WAVES && s_c1[lane & (JOIN_WAVES - 1)] != 0); runs; runs &= runs - 1) {
+      const int i = __builtin_ctzll(runs);
       const u32 b = s_c0[i], n = s_c1[i] - b;
-      if (n == 0) continue;
       acc.clear();
-      add_partials<DT>(acc, a, b, b + (u32)((u64)n * w / WAVES), b + (u32)((u64)n * (w + 1) / WAVES), col);
+      add_partials<DT>(acc, a, b, b + (u32)((u64)n * w / JOIN_WAVES), b + (u32)((u64)n * (w + 1) / JOIN_WAVES), col);
 #pragma unroll
       for (int q = 0; q < E::VEC; ++q) s_sum[w][q][lane] = acc.f[q];
       __syncthreads();
@@ -499,10 +568,10 @@ __global__ __launch_bounds__(THREADS) void embed_join_kernel(GradArgs a) {
 #pragma unroll
         for (int q = 0; q < E::VEC; ++q) {
           float x = s_sum[0][q][lane];
-          for (int k = 1; k < WAVES; ++k) x += s_sum[k][q][lane];
+          for (int k = 1; k < JOIN_WAVES; ++k) x += s_sum[k][q][lane];
           acc.f[q] = x;
         }
-        acc.store(a.dt, v * a.D, col, a.D, a.scale);
+        acc.store(a.dt, (long long)word * a.D, col, a.D, a.scale);
       }
       __syncthreads();
     }
@@ -571,11 +640,11 @@ static int chunk_of(long long N, int D) {
   return want >= 64 ? 64 : want >= 32 ? 32 : want >= 16 ? 16 : 8;
 }
 
-// key and place twice, the histograms, the runs' starts, the chunks' partial sums
+// key and place twice, the histograms, the chunks' partial sums
 extern "C" long long s2c_embed_grad_workspace_bytes(long long N, int V, int D) {
   if (N <= 0 || V <= 0 || D <= 0 || by_scan(N, V)) return 0;
   const int chunk = chunk_of(N, D);
-  return 4 * align16(4 * N) + 4LL * RADIX * MAX_SORT_GRID + align16(4 * ((long long)V + 1)) +
+  return 4 * align16(4 * N) + 4LL * RADIX * MAX_SORT_GRID +
          8 * ((N + chunk - 1) / chunk) * ((D + 7) & ~7);
 }
 
@@ -589,11 +658,13 @@ static void grad_launch(GradArgs &a, bool scan, hipStream_t st) {
     hipLaunchKernelGGL((embed_grad_scan_kernel<DT>), dim3(grid_of((units + WAVES - 1) / WAVES)), block, 0, st, a);
     return;
   }
-  const long long waves = (a.N + a.chunk - 1) / a.chunk * a.pieces, starts = ((long long)a.V + THREADS) / THREADS;
-  const int sums = grid_of((waves + WAVES - 1) / WAVES);
-  hipLaunchKernelGGL((embed_runs_kernel<DT>), dim3(sums + (int)(starts < 65536 ? starts : 65536)), block, 0, st, a, sums);
-  const long long units = ((long long)a.V + WAVES - 1) / WAVES * a.pieces;
-  hipLaunchKernelGGL((embed_join_kernel<DT>), dim3(grid_of(units)), block, 0, st, a);
+  const long long chunks = (a.N + a.chunk - 1) / a.chunk;
+  const int sums = grid_of((chunks * a.pieces + WAVES - 1) / WAVES);
+  const long long absent = ((long long)a.V + WORDS - 1) / WORDS * ((a.pieces + GROUP - 1) / GROUP);
+  hipLaunchKernelGGL((embed_runs_kernel<DT>), dim3(sums + (int)(absent < 65536 ? absent : 65536)), block, 0, st, a, sums);
+  if (chunks > 1)
+    hipLaunchKernelGGL((embed_join_kernel<DT>), dim3(min(grid_of((chunks + JOIN_WAVES - 1) / JOIN_WAVES * a.pieces), 1 << 16)),
+                       dim3(64 * JOIN_WAVES), 0, st, a);
 }
 
 static void sort_tokens(GradArgs &a, u32 *const *key, u32 *const *pos, u32 *counts, hipStream_t st) {
@@ -663,8 +734,7 @@ extern "C" int s2c_embed_grad(long long N, int V, int D, int dtype, long long ld
     }
     u32 *counts = (u32 *)p;
     p += 4LL * RADIX * MAX_SORT_GRID;
-    a.start = (u32 *)p;
-    a.partial = (float *)(p + align16(4 * ((long long)V + 1)));
+    a.partial = (float *)p;
     sort_tokens(a, key, pos, counts, st);
   }
   if (dtype == S2C_F32) grad_launch<S2C_F32>(a, scan, st);
