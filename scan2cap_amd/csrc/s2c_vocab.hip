@@ -852,8 +852,8 @@ long long vectors(int V, int dtype) {                  // of a row, at any align
 
 // How a row is shared out: `waves` of a workgroup to a stretch, `split` stretches to a row.
 //  * many rows: a wave each -- no barrier, no merge, one threshold for the whole row (59392 rows of 3500
-//    fp32 words, 5 alternatives: 161 us, against 292 us with 4 waves a row; 150 us since its row lives in
-//    scalar registers);
+//    fp32 words, 5 alternatives: 157 us; 161 before its row lived in scalar registers, against 292 with
+//    4 waves a row);
 //  * rows that would leave most of the chip empty: 16 waves (32768 bf16 words, one row: 8.0 us, 9.7 with 4,
 //    20.9 with 1), and stretches of at least one round of tiles, up to 256 workgroups, joined by a second
 //    launch (64 rows of 131072 words: 17.4 us in 4 stretches, 18.6 in one; one row of 262144 fp32 words: 14.2
