@@ -333,7 +333,10 @@ __device__ __forceinline__ Stat stream_row(const char *xr, int V, int vb, int ve
 }
 
 // ---- what is written for a row ---------------------------------------------------------------------------
-// stats: {mref, log2 s0, ., .}; log2 s0 = +inf marks a row without gradient, NaN one whose gradient is NaN
+// stats: {mref, 1 / s0, entropy, log2 s0} of scores, {mref, 1 / s0, max w, 1 / sum 2^((w - max w) c)} of
+// distillation; 1 / s0 = 0 marks a row without gradient (else s0 is at least 1, for the largest logit), NaN one
+// whose gradient is NaN.  p is formed as 2^d (1 / s0): d - log2 s0 would be rounded at its size, 10 to 25, and
+// leave up to 11 roundings in p where this leaves one.
 __device__ __forceinline__ float log2_sum(const Stat &s) {
   return s.s0 == 0.0f ? INFINITY : log2f(s.s0);        // (0: every logit is -inf)
 }
@@ -435,7 +438,7 @@ __device__ __forceinline__ void scores_write_dead(const s2c_token_scores_args &a
   if (lane == 0) {
     if (a.logp) a.logp[r] = 0.0f;
     a.entropy[r] = 0.0f;
-    if (a.stats) *reinterpret_cast<float4 *>(a.stats + 4 * (size_t)r) = make_float4(0.0f, INFINITY, 0.0f, 0.0f);
+    if (a.stats) *reinterpret_cast<float4 *>(a.stats + 4 * (size_t)r) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   }
   for (int j = lane; j < a.k; j += 64) {
     a.top_logp[(size_t)r * a.k + j] = 0.0f;
@@ -460,7 +463,7 @@ __device__ __forceinline__ void scores_write(const s2c_token_scores_args &a, int
     }
     a.entropy[r] = h < 0.0f ? 0.0f : h;
     if (a.stats) *reinterpret_cast<float4 *>(a.stats + 4 * (size_t)r) =
-        make_float4(mref, bad ? NAN : l2s, h < 0.0f ? 0.0f : h, 0.0f);
+        make_float4(mref, bad ? NAN : dead ? 0.0f : 1.0f / s.s0, h < 0.0f ? 0.0f : h, l2s);
   }
   if (lane < a.k) {
     const u64 key = top[lane];
@@ -523,7 +526,7 @@ __global__ __launch_bounds__(256) void scores_join_kernel(s2c_token_scores_args 
 struct Slots {
   long long id[SLOTS / 64];
   float lq[SLOTS / 64], q[SLOTS / 64];
-  float wm, l2w;          // l2w = +inf: no slot is used
+  float wm, l2w, inv;     // log2 of the sum and its inverse; l2w = +inf: no slot is used
 };
 
 __device__ __forceinline__ Slots load_slots(const s2c_distill_args &a, int r, float c, int lane) {
@@ -547,10 +550,11 @@ __device__ __forceinline__ Slots load_slots(const s2c_distill_args &a, int r, fl
   for (int i = 0; i < SLOTS / 64; ++i) sum += exp2_((w[i] - s.wm) * c);
   sum = wave_sum(sum);
   s.l2w = sum == 0.0f ? INFINITY : log2f(sum);
+  s.inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
   for (int i = 0; i < SLOTS / 64; ++i) {
     s.lq[i] = (w[i] - s.wm) * a.lg.inv_t - LN2 * s.l2w;
-    s.q[i] = exp2_((w[i] - s.wm) * c - s.l2w);
+    s.q[i] = exp2_((w[i] - s.wm) * c) * s.inv;
   }
   return s;
 }
@@ -558,7 +562,7 @@ __device__ __forceinline__ Slots load_slots(const s2c_distill_args &a, int r, fl
 __device__ __forceinline__ void distill_write_dead(const s2c_distill_args &a, int r, int lane) {
   if (lane == 0) {
     a.loss[r] = 0.0f;
-    if (a.stats) *reinterpret_cast<float4 *>(a.stats + 4 * (size_t)r) = make_float4(0.0f, INFINITY, 0.0f, INFINITY);
+    if (a.stats) *reinterpret_cast<float4 *>(a.stats + 4 * (size_t)r) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   }
 }
 
@@ -588,7 +592,8 @@ __device__ __forceinline__ void distill_write(const s2c_distill_args &a, int r, 
   bad = __ballot(bad) != 0;
   if (lane == 0) {
     a.loss[r] = bad ? NAN : part;
-    if (a.stats) *reinterpret_cast<float4 *>(a.stats + 4 * (size_t)r) = make_float4(mref, bad ? NAN : l2s, t.wm, t.l2w);
+    if (a.stats) *reinterpret_cast<float4 *>(a.stats + 4 * (size_t)r) =
+        make_float4(mref, bad ? NAN : l2s == INFINITY ? 0.0f : 1.0f / s.s0, t.wm, t.inv);
   }
 }
 
@@ -648,10 +653,10 @@ __global__ __launch_bounds__(256) void distill_join_kernel(s2c_distill_args a, S
 }
 
 // ---- gradients -------------------------------------------------------------------------------------------
-// dx_v = p_v (A + B max(d_v - log2 s0, D_MIN)) + the sparse entries of v:
-//   scores  A = -(g + sum g_top + g_H H) inv_t, B = -g_H ln 2 inv_t, entries g inv_t at the token and
+// dx_v = 2^d_v (A + B max(d_v, D_MIN)) + the sparse entries of v, with i = inv_t / s0:
+//   scores  A = -(g + sum g_top + g_H (H - ln 2 log2 s0)) i, B = -g_H ln 2 i, entries g inv_t at the token and
 //           g_top_j inv_t at top_ids_j
-//   distill A = g inv_t, B = 0, entries -g q_j inv_t at id_j
+//   distill A = g i, B = 0, entries -g q_j inv_t at id_j
 // A group of G waves loads its stretch of the row (U vectors a lane).  While the loads are under way its
 // first wave gathers the entries that lie in the stretch, in slot order, with their logits.  Then the dense
 // part is written, and the first entry of every word writes its element once more with all entries of
@@ -703,8 +708,8 @@ __global__ __launch_bounds__(256) void vocab_bwd_kernel(GradArgs a) {
     const long long o0 = (long long)r * V;
     const int shift = (int)((((uintptr_t)a.dx / E::ES) + o0) & (VEC - 1));       // of the stores
     const float4 st = *reinterpret_cast<const float4 *>(a.stats + 4 * (size_t)r);
-    const float mref = st.x, l2s = st.y;
-    const bool dead = l2s == INFINITY;
+    const float mref = st.x, inv = st.y;
+    const bool dead = inv == 0.0f;
     const long long b0 = (long long)seg * a.span * VEC - shift;                  // the stretch's elements
     const long long b1 = min((long long)V, b0 + (long long)a.span * VEC);
     Raw x[U];
@@ -731,13 +736,14 @@ __global__ __launch_bounds__(256) void vocab_bwd_kernel(GradArgs a) {
       float g;
       if (DISTILL) {
         n = a.K;
-        g = A = a.g_loss[r] * it;
+        g = a.g_loss[r] * it;
+        A = g * inv;
       } else {
         const float ge = a.g_entropy ? a.g_entropy[r] : 0.0f;
         g = (a.g_logp && a.token) ? a.g_logp[r] * it : 0.0f;
         n = 1 + (a.g_top ? a.k : 0);
-        A = -(ge * st.z * it);
-        B = -ge * LN2 * it;
+        A = -ge * (st.z - LN2 * st.w) * it;
+        B = -ge * LN2 * it * inv;
       }
       if (tid < 64) {
         float sum = 0.0f;
@@ -750,7 +756,7 @@ __global__ __launch_bounds__(256) void vocab_bwd_kernel(GradArgs a) {
             if (DISTILL) {
               id = a.ids[(size_t)r * n + j];
               if (id >= 0)
-                val = -g * exp2_((load_any(a.teacher, (long long)r * n + j, a.teacher_dtype) - st.z) * c - st.w);
+                val = -g * (exp2_((load_any(a.teacher, (long long)r * n + j, a.teacher_dtype) - st.z) * c) * st.w);
             } else if (j == 0) {
               id = a.token ? a.token[r] : -1;
               val = g;
@@ -778,10 +784,10 @@ __global__ __launch_bounds__(256) void vocab_bwd_kernel(GradArgs a) {
       }
     }
     group_sync<G>();
-    if (!DISTILL && !dead) A -= en.sum;
+    if (!DISTILL && !dead) A = (A - en.sum) * inv;
     auto grad = [&](float v) {
-      const float d = (v - mref) * c - l2s;
-      return exp2_(d) * __builtin_fmaf(B, fmaxf(d, D_MIN), A);
+      const float d = (v - mref) * c;
+      return exp2_(d) * (DISTILL ? A : __builtin_fmaf(B, fmaxf(d, D_MIN), A));
     };
 #pragma unroll
     for (int u = 0; u < U; ++u) {
