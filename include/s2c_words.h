@@ -65,7 +65,8 @@ int s2c_token_scores_bwd(const s2c_token_scores_args *a, const float *g_logp, co
  * id < 0 or a logit of -inf = an empty slot.  q = softmax over the used slots of teacher * inv_t,
  *   loss = sum_j q_j (log q_j - log p[id_j]),   p = softmax(x * inv_t) over all V words.
  * mask (rows bytes, may be NULL): rows with 0 are not read.  Masked rows and rows without a used slot:
- * loss 0, zero gradient.  A row of only -inf logits: loss +inf, zero gradient.  An id >= V: NaN.
+ * loss 0, zero gradient.  A row of only -inf logits: loss +inf, zero gradient.  A used slot whose id is >= V
+ * or whose logit is NaN or +inf: loss and the whole row's gradient NaN.
  * stats (rows x 4, or NULL) as above. */
 typedef struct {
   s2c_logits lg;

@@ -522,7 +522,7 @@ __global__ __launch_bounds__(256) void scores_join_kernel(s2c_token_scores_args 
 }
 
 // ---- distillation --------------------------------------------------------------------------------------
-// the teacher's softmax over a row's slots, slot j of lane l = l + 64 i: log q and q
+// the teacher's softmax over a row's slots, slot j of lane l = l + 64 i: log q and q; id -1: an empty slot
 struct Slots {
   long long id[SLOTS / 64];
   float lq[SLOTS / 64], q[SLOTS / 64];
@@ -541,6 +541,7 @@ __device__ __forceinline__ Slots load_slots(const s2c_distill_args &a, int r, fl
     if (j < a.K) {
       s.id[i] = a.ids[(size_t)r * a.K + j];
       if (s.id[i] >= 0) w[i] = load_any(a.teacher, (long long)r * a.K + j, a.teacher_dtype);
+      if (w[i] == -INFINITY) s.id[i] = -1;
     }
     m = nan_max(m, w[i]);
   }
@@ -580,13 +581,12 @@ __device__ __forceinline__ void distill_write(const s2c_distill_args &a, int r, 
   const float l2s = log2_sum(s);
   const float sub = l2s == INFINITY ? 0.0f : l2s;
   float part = 0.0f;
-  bool bad = false;
+  bool bad = t.l2w != t.l2w;                    // (a teacher's NaN or +inf)
 #pragma unroll
   for (int i = 0; i < SLOTS / 64; ++i) {
-    if (t.q[i] != 0.0f) {                       // (empty slots and vanishing ones add nothing; NaN does)
-      if (t.id[i] >= a.lg.V) bad = true;
-      else part += t.q[i] * (t.lq[i] - ((at[i] - mref) * a.lg.inv_t - LN2 * sub));
-    }
+    if (t.id[i] >= a.lg.V) bad = true;
+    else if (t.q[i] != 0.0f)                    // (empty slots and vanishing ones add nothing)
+      part += t.q[i] * (t.lq[i] - ((at[i] - mref) * a.lg.inv_t - LN2 * sub));
   }
   part = wave_sum(part);
   bad = __ballot(bad) != 0;

@@ -85,8 +85,8 @@ def distill_loss(logits, teacher_ids, teacher_logits, temperature=1.0, mask=None
     Log probabilities serve as teacher logits as well (`token_scores(...).top_ids / .top_logp` of the
     teacher).  A slot with a negative id or a logit of -inf is empty; an id may occur twice.  Rows with
     mask (..., bool) False are not read; they and rows without a used slot have loss 0 and zero gradient.
-    A used id >= V makes the row's loss and gradient NaN; a row of logits that are all -inf has loss +inf
-    and zero gradient."""
+    A used slot with an id >= V (whatever its weight) or a logit of NaN or +inf makes the row's loss and whole
+    gradient NaN; a row of logits that are all -inf has loss +inf and zero gradient."""
     try:
         return _ext.distill_loss(logits, teacher_ids, teacher_logits, temperature, mask)
     except TypeError:

@@ -30,3 +30,37 @@ def test_gradients_of_uniform_rows_carry_one_rounding(rows, V, T):
     want[ids[0, :3]] -= 1 / (3 * T)
     # the slots: a rounding of 1 / 3, one of the sum
     assert bool(((dx.double() - want).abs() <= 3 * U * want.abs()).all())
+
+
+@pytest.mark.parametrize("rows,V", [(20, 70), (8, 140000), (300, 3500), (2100, 1000)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_a_bad_teacher_slot_makes_the_whole_row_nan(rows, V, dtype):
+    """NaN or +inf among a row's used slots, or a used word outside the vocabulary, however small its weight: loss and
+    every element of the gradient NaN; the same in empty slots and masked rows: no trace, and none in other rows."""
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    x = torch.randn(rows, V, generator=g, device="cuda").to(dtype)
+    ids = torch.randint(0, V, (rows, 5), generator=g, device="cuda")
+    w = torch.randn(rows, 5, generator=g, device="cuda")
+    good_ids, good_w = ids.clone(), w.clone()
+    w[0, 2] = float("nan")
+    w[1, 4] = float("inf")
+    w[2] = float("inf")
+    ids[3, 1] = V
+    ids[4, 1], w[4, 1] = V + 5, -1000.0                       # 2^-1443 of the weight
+    ids[5, 0], w[5, 0] = -1, float("nan")
+    good_ids[5, 0] = -1
+    ids[6, 3], w[6, 3] = 2 ** 40, float("-inf")
+    good_ids[6, 3] = -1
+    w[7, 0] = float("nan")
+    mask = torch.ones(rows, dtype=torch.bool, device="cuda")
+    mask[7] = False
+    out = []
+    for i, t in ((ids, w), (good_ids, good_w)):
+        leaf = x.clone().requires_grad_()
+        loss = word_ops.distill_loss(leaf, i, t, temperature=1.5, mask=mask)
+        dx, = torch.autograd.grad([loss], [leaf], [torch.ones_like(loss)])
+        out.append((loss.detach(), dx))
+    (loss, dx), (want, want_dx) = out
+    assert bool(loss[:5].isnan().all()) and bool(dx[:5].isnan().all())
+    assert torch.equal(loss[5:], want[5:]) and torch.equal(dx[5:], want_dx[5:])
+    assert bool(want.isfinite().all()) and loss[7].item() == 0 and bool((dx[7] == 0).all())
