@@ -82,7 +82,8 @@ int s2c_distill_fwd(const s2c_distill_args *a, void *stream);
 /* dx (rows, V) contiguous: dx_v = g (p_v sum_j q_j - sum_{j: id_j = v} q_j) inv_t */
 int s2c_distill_bwd(const s2c_distill_args *a, const float *g_loss, void *dx, void *stream);
 
-/* size of s2c_logits (0), s2c_token_scores_args (1), s2c_distill_args (2) as compiled */
+/* size of s2c_logits (0), s2c_token_scores_args (1), s2c_distill_args (2) as compiled: a caller that was built
+ * apart from the library compares them with its own before its first call */
 long long s2c_words_args_sizeof(int which);
 
 /* out (N, D) contiguous = scale * table[token] (table (V, D): unit column stride, row stride `ld`

@@ -434,6 +434,12 @@ Tensor embed_tokens(const Tensor &tokens, const Tensor &table, double scale, std
 }  // namespace
 
 PYBIND11_MODULE(s2c_words_ext, m) {
+  // the argument blocks of the library that is loaded, against those that this file was compiled with
+  const long long sizes[] = {sizeof(s2c_logits), sizeof(s2c_token_scores_args), sizeof(s2c_distill_args)};
+  for (int i = 0; i < 3; ++i)
+    if (s2c_words_args_sizeof(i) != sizes[i])
+      throw py::import_error("s2c_words_ext.so and libs2c_hip.so were built from different headers -- run "
+                             "`python -m scan2cap_amd.build`");
   m.def("token_scores", &token_scores);
   m.def("distill_loss", &distill_loss);
   m.def("embed_tokens", &embed_tokens);
