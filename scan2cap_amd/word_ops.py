@@ -47,11 +47,16 @@ def _load():
 _ext = _load()
 
 
-def _refuse(**tensors):
-    """After a TypeError of the binding: say which argument is no tensor."""
+def _refuse(numbers, **tensors):
+    """After a TypeError of the binding: say which argument is no tensor, or what the other arguments are."""
     for name, t in tensors.items():
         if not torch.is_tensor(t):
             raise ValueError("%s must be a tensor, not %s" % (name, type(t).__name__)) from None
+    raise ValueError("numbers of a wrong type or out of range: %r" % (numbers,)) from None
+
+
+def _given(**tensors):
+    return {name: t for name, t in tensors.items() if t is not None}
 
 
 def token_scores(logits, tokens=None, top_k=0, temperature=1.0, ignore_index=None):
@@ -72,8 +77,8 @@ def token_scores(logits, tokens=None, top_k=0, temperature=1.0, ignore_index=Non
     try:
         return TokenScores._make(_ext.token_scores(logits, tokens, top_k, temperature, ignore_index))
     except TypeError:
-        _refuse(logits=logits)
-        raise
+        _refuse(dict(top_k=top_k, temperature=temperature, ignore_index=ignore_index), logits=logits,
+                **_given(tokens=tokens))
 
 
 def distill_loss(logits, teacher_ids, teacher_logits, temperature=1.0, mask=None):
@@ -90,8 +95,8 @@ def distill_loss(logits, teacher_ids, teacher_logits, temperature=1.0, mask=None
     try:
         return _ext.distill_loss(logits, teacher_ids, teacher_logits, temperature, mask)
     except TypeError:
-        _refuse(logits=logits, teacher_ids=teacher_ids, teacher_logits=teacher_logits)
-        raise
+        _refuse(dict(temperature=temperature), logits=logits, teacher_ids=teacher_ids, teacher_logits=teacher_logits,
+                **_given(mask=mask))
 
 
 def embed_tokens(tokens, table, scale=1.0, padding_idx=None):
@@ -103,5 +108,4 @@ def embed_tokens(tokens, table, scale=1.0, padding_idx=None):
     try:
         return _ext.embed_tokens(tokens, table, scale, padding_idx)
     except TypeError:
-        _refuse(tokens=tokens, table=table)
-        raise
+        _refuse(dict(scale=scale, padding_idx=padding_idx), tokens=tokens, table=table)

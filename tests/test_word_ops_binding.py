@@ -1,9 +1,14 @@
-"""The word operators' torch binding beside a kernel library of other headers, on the CPU."""
+"""The word operators' torch binding on the CPU: beside a kernel library of other headers, and its answer to
+arguments of types that it does not take."""
 import os
 import subprocess
 import sys
 
+import pytest
+import torch
+
 from tests import words_common  # noqa: F401  (first: the binding)
+from scan2cap_amd import word_ops
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -19,3 +24,21 @@ def test_a_library_of_other_headers_is_refused(tmp_path):
                         "except ImportError as e:\n    print(e)\n")
         out = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
         assert said in out.stdout, (out.stdout, out.stderr)
+
+
+_X, _T = torch.zeros(2, 5), torch.zeros(2, dtype=torch.int64)
+
+
+@pytest.mark.parametrize("said,call", [
+    ("tokens must be a tensor, not list", lambda: word_ops.token_scores(_X, [0, 1])),
+    ("top_k", lambda: word_ops.token_scores(_X, _T, top_k=1.5)),
+    ("temperature", lambda: word_ops.token_scores(_X, _T, temperature=None)),
+    ("ignore_index", lambda: word_ops.token_scores(_X, _T, ignore_index=0.5)),
+    ("mask must be a tensor, not list", lambda: word_ops.distill_loss(_X, _T[:, None], _X[:, :1], mask=[True, False])),
+    ("temperature", lambda: word_ops.distill_loss(_X, _T[:, None], _X[:, :1], temperature="2")),
+    ("scale", lambda: word_ops.embed_tokens(_T, _X, scale=None)),
+    ("padding_idx", lambda: word_ops.embed_tokens(_T, _X, padding_idx=2 ** 70)),
+])
+def test_arguments_of_other_types_are_value_errors(said, call):
+    with pytest.raises(ValueError, match=said):
+        call()
