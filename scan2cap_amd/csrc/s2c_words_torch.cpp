@@ -65,9 +65,13 @@ void check_gpu(const char *name, const Tensor &t, const Tensor &like) {
   check_place(t.device() == like.device(), name, " is on ", t.device(), ", the other tensors on ", like.device());
 }
 
+// values that memory holds as they are (the imaginary part of a conjugated tensor is a view whose sign is
+// applied by whoever reads it)
+Tensor as_stored(const Tensor &t) { return t.is_neg() ? t.resolve_neg() : t; }
+
 // (the usual case costs no dispatch)
 Tensor dense(const Tensor &t, at::ScalarType type) {
-  return t.scalar_type() == type && t.is_contiguous() ? t : t.to(type).contiguous();
+  return t.scalar_type() == type && t.is_contiguous() ? as_stored(t) : as_stored(t.to(type).contiguous());
 }
 
 Tensor ids64(const Tensor &t) { return dense(t, at::kLong); }
@@ -111,7 +115,8 @@ Axes merge_axes(const Tensor &x, int64_t dims) {
 
 // Up to three leading axes of any strides are read in place (a decoder's word-major logits permuted to
 // (B, K, T, V)); more, or words that are not adjacent, are copied first.
-Tensor readable(const Tensor &x) {
+Tensor readable(const Tensor &t) {
+  const Tensor x = as_stored(t);
   const bool adjacent = x.size(-1) == 1 || x.stride(-1) == 1;
   return adjacent && merge_axes(x, x.dim() - 1).n <= 3 ? x : x.contiguous();
 }
@@ -357,7 +362,7 @@ Tensor distill_loss(const Tensor &logits, const Tensor &ids, const Tensor &teach
   check_gpu("teacher_ids", ids, logits);
   check_gpu("teacher_logits", teacher, logits);
   if (mask.has_value()) check_gpu("mask", *mask, logits);
-  const Tensor i = ids64(ids), w = teacher.detach().contiguous();
+  const Tensor i = ids64(ids), w = dense(teacher.detach(), teacher.scalar_type());
   const MaybeTensor m = mask.has_value() ? MaybeTensor(mask->contiguous()) : MaybeTensor();
   if (!wants_grad(logits))
     return distill_forward(readable(logits), i, w, m.value_or(Tensor()), temperature, false).loss;
@@ -386,13 +391,13 @@ struct EmbedFn : torch::autograd::Function<EmbedFn> {
     ctx->saved_data["V"] = table.size(0);
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["padding"] = padding;
-    return embed_forward(tokens, table, scale, padding);
+    return embed_forward(tokens, as_stored(table), scale, padding);
   }
 
   static variable_list backward(AutogradContext *ctx, const variable_list &grads) {
     variable_list out(4);
-    Tensor g = grads[0];
-    if (!g.defined()) return out;
+    if (!grads[0].defined()) return out;
+    Tensor g = as_stored(grads[0]);
     const c10::DeviceGuard guard(g.device());
     const Tensor tokens = ctx->get_saved_variables()[0];
     const int64_t N = tokens.numel(), V = ctx->saved_data["V"].toInt(), D = g.size(-1);
@@ -428,7 +433,7 @@ Tensor embed_tokens(const Tensor &tokens, const Tensor &table, double scale, std
   const Tensor t = ids64(tokens);
   check(padding != std::optional<int64_t>(S2C_WORDS_NO_PADDING), "padding_idx cannot be the lowest integer");
   const int64_t pad = padding.value_or(S2C_WORDS_NO_PADDING);
-  return wants_grad(table) ? EmbedFn::apply(t, table, scale, pad) : embed_forward(t, table, scale, pad);
+  return wants_grad(table) ? EmbedFn::apply(t, table, scale, pad) : embed_forward(t, as_stored(table), scale, pad);
 }
 
 }  // namespace

@@ -64,3 +64,36 @@ def test_a_bad_teacher_slot_makes_the_whole_row_nan(rows, V, dtype):
     assert bool(loss[:5].isnan().all()) and bool(dx[:5].isnan().all())
     assert torch.equal(loss[5:], want[5:]) and torch.equal(dx[5:], want_dx[5:])
     assert bool(want.isfinite().all()) and loss[7].item() == 0 and bool((dx[7] == 0).all())
+
+
+def _negated_view(t):
+    """A real tensor of t's values whose memory holds their negatives."""
+    v = torch.complex(torch.zeros_like(t), -t).conj().imag
+    assert v.is_neg() and torch.equal(v, t)
+    return v
+
+
+def test_lazily_negated_tensors():
+    """The imaginary part of a conjugated tensor (its sign is applied when it is read) in every place."""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    n = lambda *s: torch.randn(*s, generator=g, device="cuda")                  # noqa: E731
+    x, w, table = n(6, 90), n(6, 3), n(90, 8)
+    t = torch.randint(0, 90, (6,), generator=g, device="cuda")
+    ids = torch.randint(0, 90, (6, 3), generator=g, device="cuda")
+    up, up_y = n(6), n(6, 8)
+    got, want = [], []
+    for out, f in ((want, lambda v: v), (got, _negated_view)):
+        for train in (False, True):
+            a = f(x).detach().requires_grad_(train)
+            # (columns beside each other: every second float, as an imaginary part lies, is refused for a table)
+            b = (table if f(x) is x else torch._neg_view(-table)).detach().requires_grad_(train)
+            y = [word_ops.token_scores(a, t, top_k=4).logp, word_ops.distill_loss(a, ids, f(w)),
+                 word_ops.embed_tokens(t, b, scale=2.0)]
+            out += y
+            if train:
+                for o, leaf, u in zip(y, (a, a, b), (up, up, up_y)):
+                    out += torch.autograd.grad([o], [leaf], [f(u)])
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    with pytest.raises(ValueError, match="adjacent"):
+        word_ops.embed_tokens(t, _negated_view(table))
