@@ -152,11 +152,17 @@ def _embedding_table(vocabulary, embeddings, emb_size):
 def _word_embs(module, data_dict):
     """The captions' word embeddings (B,T,emb): `lang_feat` where the caller brought it (the reference's
     dataset looks every word up on the host, lib/dataset.py:184-199), else the table's rows of `lang_ids` on
-    the device, zeros at padding (word 0) -- 8 bytes a word to copy instead of 1200, and a gradient for a
-    table that `learn_word_embeddings` has made a parameter."""
-    if "lang_feat" in data_dict:
+    the device, zeros at padding (word 0) -- 8 bytes a word to copy instead of 1200.  A table that
+    `learn_word_embeddings` has made a parameter is looked up in any case: `lang_feat` holds rows of the table
+    as it was, through which it would never train."""
+    table = module._emb_table
+    learned = isinstance(table, nn.Parameter)
+    if "lang_feat" in data_dict and not learned:
         return data_dict["lang_feat"]
-    ids, table = data_dict["lang_ids"], module._emb_table
+    ids = data_dict.get("lang_ids")
+    if ids is None:
+        raise ValueError("the batch has no lang_ids, in which %s" % (
+            "learned word embeddings are looked up" if learned else "the words are looked up where it has no lang_feat"))
     if table.is_cuda:
         from ..word_ops import embed_tokens
         return embed_tokens(ids, table, padding_idx=0)
@@ -165,7 +171,8 @@ def _word_embs(module, data_dict):
 
 def _learn_word_embeddings(module):
     """Make the captioner's embedding table a parameter (`_emb_table`, in `state_dict()` from then on), so that
-    it trains with the rest when `lang_feat` is not given."""
+    it trains with the rest.  The words of every batch are then its rows of `lang_ids`, whether the batch has a
+    `lang_feat` or not."""
     if not isinstance(module._emb_table, nn.Parameter):
         table = module._emb_table
         del module._emb_table
