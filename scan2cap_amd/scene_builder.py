@@ -453,16 +453,20 @@ class SceneBatchBuilder(object):
 class AnnotationTable(object):
     """The language side of an item (lib/dataset.py:326-329, :505-508, :531-534) served
     from resident tensors: `lang_feat` (A,32,300) f32, `lang_ids` (A,32) i64, `lang_len`
-    (A) i64 (already clipped to MAX_DES_LEN + 2), plus per-annotation integers."""
+    (A) i64 (already clipped to MAX_DES_LEN + 2), plus per-annotation integers.
+    lang_feat None: the batches have none, and the captioner looks the words up in its table
+    by `lang_ids` (0.3 KB an annotation in place of 38.7; the table may be learned)."""
 
     def __init__(self, device, lang_feat, lang_ids, lang_len, object_id, ann_id,
                  object_cat, unique_multiple):
         dev = torch.device(device)
         t = lambda a, dt: torch.as_tensor(np.asarray(a), dtype=dt).to(dev)
-        self.t = {"lang_feat": t(lang_feat, torch.float32), "lang_ids": t(lang_ids, torch.int64),
+        self.t = {"lang_ids": t(lang_ids, torch.int64),
                   "lang_len": t(lang_len, torch.int64), "object_id": t(object_id, torch.int64),
                   "ann_id": t(ann_id, torch.int64), "object_cat": t(object_cat, torch.int64),
                   "unique_multiple": t(unique_multiple, torch.int64)}
+        if lang_feat is not None:
+            self.t["lang_feat"] = t(lang_feat, torch.float32)
         self.object_id_host = np.asarray(object_id, np.int64)
         self.device = dev
         self._upload = _SmallUploads(dev)
@@ -496,6 +500,10 @@ class BatchFeeder(object):
         training stream (pipeline.independent_streams) -- the producer parks on an event
         until the previous reader of a buffer set is done, and a parked stream holds up
         every other stream mapped to the same queue."""
+        served = getattr(annotations, "t", None)
+        if served is not None and "lang_feat" not in served \
+                and any(torch.is_tensor(b.get("lang_feat")) for b in buffers):
+            raise ValueError("a buffer set has a lang_feat, which annotations without one would leave stale")
         self.builder, self.annotations, self.buffers = builder, annotations, buffers
         self.device_choices = device_choices
         self.rng = rng if rng is not None else np.random.RandomState(0)

@@ -48,3 +48,34 @@ def test_words_need_ids_or_features(kind):
     mod.learn_word_embeddings()
     with pytest.raises(ValueError, match="learned word embeddings"):
         mod(dict(feat_only))
+
+
+def _annotations(device, dd, feat):
+    from scan2cap_amd.scene_builder import AnnotationTable
+    n = pc.B
+    return AnnotationTable(device, dd["lang_feat"].cpu().numpy() if feat else None, dd["lang_ids"].cpu().numpy(),
+                           dd["lang_len"].cpu().numpy(), [4] * n, [0] * n, [2] * n, [0] * n)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_annotations_without_features_feed_the_captioner(device):
+    dd, vocabulary, embeddings = _batch(device)
+    mod = _module("topdown", device, vocabulary, embeddings)
+    picks = [1, 0]
+    with_feat, without = (_annotations(device, dd, feat).gather(picks) for feat in (True, False))
+    assert set(with_feat) - set(without) == {"lang_feat"}
+    for k in without:
+        assert torch.equal(with_feat[k], without[k])
+    rest = {k: v for k, v in dd.items() if not k.startswith("lang_")}
+    a, b = (mod(dict(rest, **batch))["lang_cap"] for batch in (with_feat, without))
+    assert torch.equal(a, b)
+
+
+def test_a_feeder_leaves_no_stale_features():
+    from scan2cap_amd.scene_builder import BatchFeeder
+    dd, _, _ = _batch("cpu")
+    anns = _annotations("cpu", dd, False)
+    with pytest.raises(ValueError, match="stale"):
+        BatchFeeder(None, anns, [{"lang_ids": dd["lang_ids"]}, dict(dd)], stream=object())
+    BatchFeeder(None, anns, [{"lang_ids": dd["lang_ids"]}], stream=object())
+    BatchFeeder(None, _annotations("cpu", dd, True), [dict(dd)], stream=object())
