@@ -107,8 +107,15 @@ def load_optimizer_state_inplace(optimizer, state_dict):
 
 
 def load_checkpoint(root, model, optimizer, map_location=None, inplace=False):
-    """scripts/train.py:138-145.  Returns (epoch, best)."""
+    """scripts/train.py:138-145.  Returns (epoch, best).  Nothing is loaded where one side has learned word
+    embeddings and the other has not: the optimizer's state would not fit (`model.load_state_dict` takes either)."""
     ckpt = torch.load(os.path.join(root, "checkpoint.tar"), map_location=map_location)
+    saved, have = (any(k.split(".")[-1] == "_emb_table" for k in state)
+                   for state in (ckpt["model_state_dict"], model.state_dict()))
+    if saved != have:
+        raise ValueError("the checkpoint has %s word embeddings, the model %s: %s" % (
+            ("learned", "has not", "call learn_word_embeddings() before its optimizer is built") if saved else
+            ("no learned", "has", "resume without them, then call learn_word_embeddings() and build a new optimizer")))
     model.load_state_dict(ckpt["model_state_dict"])
     if inplace:
         load_optimizer_state_inplace(optimizer, ckpt["optimizer_state_dict"])

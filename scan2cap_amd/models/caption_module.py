@@ -169,15 +169,30 @@ def _word_embs(module, data_dict):
     return table[ids] * (ids != 0).unsqueeze(-1).to(table.dtype)
 
 
-def _learn_word_embeddings(module):
-    """Make the captioner's embedding table a parameter (`_emb_table`, in `state_dict()` from then on), so that
-    it trains with the rest.  The words of every batch are then its rows of `lang_ids`, whether the batch has a
-    `lang_feat` or not."""
-    if not isinstance(module._emb_table, nn.Parameter):
-        table = module._emb_table
-        del module._emb_table
-        module._emb_table = nn.Parameter(table.detach().clone())
-    return module
+class _WordTable(nn.Module):
+    """A captioner's embedding table `_emb_table`: a buffer outside the state_dict, or a parameter."""
+
+    def learn_word_embeddings(self):
+        """Make the embedding table a parameter, in place and in `state_dict()` from then on, so that it trains
+        with the rest.  The words of every batch are then its rows of `lang_ids`, whether the batch has a
+        `lang_feat` or not.  To be called before what collects the parameters is built (optimizer, gradient
+        buffers, captured steps): these would leave the table out."""
+        if not isinstance(self._emb_table, nn.Parameter):
+            table = self._emb_table
+            del self._emb_table
+            self._emb_table = nn.Parameter(table.detach())
+        return self
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys,
+                              unexpected_keys, error_msgs):
+        """A state_dict with a learned table makes this one a parameter too; one without leaves it as it is."""
+        key = prefix + "_emb_table"
+        if key in state_dict:
+            self.learn_word_embeddings()
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys,
+                                      unexpected_keys, error_msgs)
+        if key in missing_keys:
+            missing_keys.remove(key)
 
 
 _C.register("s2c_good_bbox_stats", [_I, _P, _F32, _P, _P, _P])
@@ -199,7 +214,7 @@ def _good_bbox_stats(target_ious, min_iou):
     return good, torch.where(n > 0, mean, torch.zeros_like(mean))
 
 
-class SceneCaptionModule(nn.Module):
+class SceneCaptionModule(_WordTable):
     """Plain GRU captioner (no attention), caption_module.py:40-200."""
 
     def __init__(self, vocabulary, embeddings, emb_size=300, feat_size=128,
@@ -216,8 +231,6 @@ class SceneCaptionModule(nn.Module):
         self.register_buffer("_emb_table",
                              _embedding_table(vocabulary, embeddings, emb_size),
                              persistent=False)
-
-    learn_word_embeddings = _learn_word_embeddings
 
     def step(self, step_input, hidden):
         hidden = self.recurrent_cell(step_input, hidden)
@@ -271,7 +284,7 @@ class SceneCaptionModule(nn.Module):
         return data_dict
 
 
-class TopDownSceneCaptionModule(nn.Module):
+class TopDownSceneCaptionModule(_WordTable):
     def __init__(self, vocabulary, embeddings, emb_size=300, feat_size=128,
                  hidden_size=512, num_proposals=256, num_locals=-1,
                  query_mode="corner", use_relation=False, use_oracle=False):
@@ -301,8 +314,6 @@ class TopDownSceneCaptionModule(nn.Module):
         self.register_buffer("_emb_table",
                              _embedding_table(vocabulary, embeddings, emb_size),
                              persistent=False)
-
-    learn_word_embeddings = _learn_word_embeddings
 
     # ---- one recurrent step ------------------------------------------------
     def _step(self, step_input, target_feat, obj_feats, hidden_1, hidden_2,
