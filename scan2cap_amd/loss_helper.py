@@ -183,7 +183,11 @@ def _trained_words(data_dict):
 def attach_teacher(data_dict, teacher_dict, top_k=16):
     """Put a teacher's best alternatives for every word into `data_dict` for `compute_cap_distill_loss`:
     `teacher_top_ids` (B,T-1,top_k) int64 and `teacher_top_logits` (their log probabilities), from the
-    `lang_cap` logits of `teacher_dict` (the same batch run through the teacher, teacher-forced)."""
+    `lang_cap` logits of `teacher_dict` (the same batch run through the teacher, teacher-forced, in a dict of its
+    own: a model writes its results into the one that it is given)."""
+    if teacher_dict is data_dict or teacher_dict["lang_cap"] is data_dict.get("lang_cap"):
+        raise ValueError("the teacher's results stand in the student's data_dict: run it on a dict of its own, "
+                         "teacher(dict(batch)), before the student's")
     logits = teacher_dict["lang_cap"].detach()
     if logits.is_cuda:
         from . import word_ops
