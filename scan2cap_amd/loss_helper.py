@@ -180,6 +180,14 @@ def _trained_words(data_dict):
     return targets
 
 
+def _log_probs(logits, live):
+    """log_softmax of the rows that are `live`, plainly, with the kernels' answers: the other rows leave no trace
+    (also where they hold NaN), a row of nothing but -inf is -inf throughout and has no gradient."""
+    none = (logits == float("-inf")).all(-1, keepdim=True)
+    x = torch.where(live.unsqueeze(-1) & ~none, logits, torch.zeros_like(logits))
+    return F.log_softmax(x, -1).masked_fill(none, float("-inf"))
+
+
 def attach_teacher(data_dict, teacher_dict, top_k=16):
     """Put a teacher's best alternatives for every word into `data_dict` for `compute_cap_distill_loss`:
     `teacher_top_ids` (B,T-1,top_k) int64 and `teacher_top_logits` (their log probabilities), from the
@@ -194,7 +202,7 @@ def attach_teacher(data_dict, teacher_dict, top_k=16):
         best = word_ops.token_scores(logits, top_k=top_k)
         data_dict["teacher_top_ids"], data_dict["teacher_top_logits"] = best.top_ids, best.top_logp
     else:
-        logp = F.log_softmax(logits, -1)
+        logp = _log_probs(logits, torch.ones_like(logits[..., 0], dtype=torch.bool))
         ids = torch.sort(logits, dim=-1, descending=True, stable=True)[1][..., :top_k]
         data_dict["teacher_top_ids"], data_dict["teacher_top_logits"] = ids, torch.gather(logp, -1, ids)
     return data_dict
@@ -211,13 +219,14 @@ def compute_cap_distill_loss(data_dict, temperature=2.0):
         from . import word_ops
         kd = word_ops.distill_loss(logits, ids, teacher.detach(), temperature=temperature, mask=rows)
     else:
-        used = ids >= 0
-        w = (teacher.detach() / temperature).masked_fill(~used, float("-inf"))
+        w = teacher.detach() / temperature
+        used = (ids >= 0) & (w != float("-inf"))
         live = rows & used.any(-1)
-        logq = F.log_softmax(torch.where(live.unsqueeze(-1), w, torch.zeros_like(w)), -1)
-        at = torch.gather(F.log_softmax(logits / temperature, -1), -1, ids.clamp(min=0))
+        w = torch.where(live.unsqueeze(-1), w.masked_fill(~used, float("-inf")), torch.zeros_like(w))
+        logq = F.log_softmax(w, -1)
+        at = torch.gather(_log_probs(logits / temperature, live), -1, torch.where(used, ids, torch.zeros_like(ids)))
         q = logq.exp()
-        terms = torch.where(q > 0, q * (logq.clamp(min=-1e30) - at), torch.zeros_like(q))
+        terms = torch.where(q != 0, q * (logq.clamp(min=-1e30) - at), torch.zeros_like(q))
         kd = torch.where(live, terms.sum(-1), torch.zeros_like(terms[..., 0]))
     return temperature ** 2 * kd.sum() / (rows.sum() + 1e-6)
 
@@ -231,7 +240,8 @@ def caption_log_likelihood(data_dict, temperature=1.0):
         from . import word_ops
         logp = word_ops.token_scores(logits, targets, temperature=temperature, ignore_index=0).logp
     else:
-        logp = torch.gather(F.log_softmax(logits / temperature, -1), -1, targets.unsqueeze(-1)).squeeze(-1)
+        logp = _log_probs(logits / temperature, targets != 0)
+        logp = torch.gather(logp, -1, targets.unsqueeze(-1)).squeeze(-1)
         logp = torch.where(targets != 0, logp, torch.zeros_like(logp))
     return logp.sum(-1), logp
 
