@@ -333,10 +333,10 @@ __device__ __forceinline__ Stat stream_row(const char *xr, int V, int vb, int ve
 }
 
 // ---- what is written for a row ---------------------------------------------------------------------------
-// stats: {mref, 1 / s0, entropy, log2 s0} of scores, {mref, 1 / s0, max w, 1 / sum 2^((w - max w) c)} of
-// distillation; 1 / s0 = 0 marks a row without gradient (else s0 is at least 1, for the largest logit), NaN one
-// whose gradient is NaN.  p is formed as 2^d (1 / s0): d - log2 s0 would be rounded at its size, 10 to 25, and
-// leave up to 11 roundings in p where this leaves one.
+// stats: {mref, s0, entropy, log2 s0} of scores, {mref, s0, max w, 1 / sum 2^((w - max w) c)} of distillation;
+// s0 = 0 marks a row without gradient (else it is at least 1, for the largest logit), NaN one whose gradient is
+// NaN.  Backward, p is formed as 2^d (1 / s0): d - log2 s0 would be rounded at its size, 10 to 25, and leave up to
+// 11 roundings in p where this leaves one.
 __device__ __forceinline__ float log2_sum(const Stat &s) {
   return s.s0 == 0.0f ? INFINITY : log2f(s.s0);        // (0: every logit is -inf)
 }
@@ -463,7 +463,7 @@ __device__ __forceinline__ void scores_write(const s2c_token_scores_args &a, int
     }
     a.entropy[r] = h < 0.0f ? 0.0f : h;
     if (a.stats) *reinterpret_cast<float4 *>(a.stats + 4 * (size_t)r) =
-        make_float4(mref, bad ? NAN : dead ? 0.0f : 1.0f / s.s0, h < 0.0f ? 0.0f : h, l2s);
+        make_float4(mref, bad ? NAN : s.s0, h < 0.0f ? 0.0f : h, l2s);
   }
   if (lane < a.k) {
     const u64 key = top[lane];
@@ -593,7 +593,7 @@ __device__ __forceinline__ void distill_write(const s2c_distill_args &a, int r, 
   if (lane == 0) {
     a.loss[r] = bad ? NAN : part;
     if (a.stats) *reinterpret_cast<float4 *>(a.stats + 4 * (size_t)r) =
-        make_float4(mref, bad ? NAN : l2s == INFINITY ? 0.0f : 1.0f / s.s0, t.wm, t.inv);
+        make_float4(mref, bad ? NAN : s.s0, t.wm, t.inv);
   }
 }
 
@@ -708,8 +708,8 @@ __global__ __launch_bounds__(256) void vocab_bwd_kernel(GradArgs a) {
     const long long o0 = (long long)r * V;
     const int shift = (int)((((uintptr_t)a.dx / E::ES) + o0) & (VEC - 1));       // of the stores
     const float4 st = *reinterpret_cast<const float4 *>(a.stats + 4 * (size_t)r);
-    const float mref = st.x, inv = st.y;
-    const bool dead = inv == 0.0f;
+    const float mref = st.x, inv = 1.0f / st.y;
+    const bool dead = st.y == 0.0f;
     const long long b0 = (long long)seg * a.span * VEC - shift;                  // the stretch's elements
     const long long b1 = min((long long)V, b0 + (long long)a.span * VEC);
     Raw x[U];
