@@ -14,7 +14,7 @@
 //    long run (10^6 x 256 bf16 whose most frequent word takes 4 %: 30 us, 73 with 4).  The rows of the
 //    words that are not in the batch are written beside the sums.
 // Measured (kernel times, MI355X): 131072 tokens x 1024 bf16, 50001 words: lookup 80 us (4.1 TB/s),
-// gradient 120 us = sort 28 + runs 82 + join 10 (floor 73 us at 5.1 TB/s); 8191 x 515 fp16, 10007 words:
+// gradient 120 us = sort 27 + runs 83 + join 10 (floor 73 us at 5.1 TB/s); 8191 x 515 fp16, 10007 words:
 // lookup 5.7 us, gradient 35 us = sort 18 + 10 + 7.
 #include "s2c_words_common.h"
 
@@ -405,8 +405,8 @@ __device__ __forceinline__ u64 present_words(const GradArgs &a, u32 v0, int lane
 }
 
 // The rows of the words that are not in the batch.  A wave writes few of them, one after the other: 64 words to
-// a workgroup take longer where the table is small (3500 rows of 8 KB: runs 24 us, 22 with 32), 8 where it is
-// large (131072 rows of 1 KB: 36 us, 22).
+// a workgroup take longer where the table is small (8192 tokens, 3500 rows of 8 KB: runs 24 us, 22 with 32), 8 where
+// it is large (2048 tokens, 131072 rows of 1 KB: 36 us, 22).
 template <int DT>
 __device__ __forceinline__ void absent_rows(const GradArgs &a, long long first, long long step) {
   const int lane = lane_id(), w = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -604,8 +604,8 @@ extern "C" int s2c_embed_fwd(long long N, int V, int D, int dtype, long long ld,
   int lpr = 1;
   while (lpr < 64 && lpr * vec < D) lpr *= 2;
   hipStream_t st = (hipStream_t)stream;
-  // an output that the 256 MB cache cannot hold is stored past it, in whole vectors (131072 x 4096 bf16: 223 us,
-  // 262 us through it; and what runs next finds no lines to be written back)
+  // an output that the 256 MB cache cannot hold is stored past it, in whole vectors (131072 x 4096 bf16: 228 us,
+  // 258 us through it; and what runs next finds no lines to be written back)
   const long long row_bytes = (long long)D * (dtype == S2C_F32 ? 4 : 2);
   const bool past_cache = N * row_bytes >= (256LL << 20) && row_bytes % 16 == 0 && ((uintptr_t)out & 15) == 0;
   auto go = [&](auto dt, auto rows) {
@@ -614,8 +614,10 @@ extern "C" int s2c_embed_fwd(long long N, int V, int D, int dtype, long long ld,
                        st, N, V, D, ld, token, table, scale, padding, out, lpr, past_cache);
   };
   auto by_rows = [&](auto dt) {
-    // many rows: a lane has 4 of them under way (131072 rows of 2 KB: 58 us, 65 with one; 10^6 of 512 bytes:
-    // 133 us, 153), else as many waves as there are (32768 rows of 2 KB: 15.6 us, 17.1 with four)
+    // many rows: a lane has 4 of them under way (in a training step, 131072 rows of 2 KB from a table of 3500 rows:
+    // 59 us, 68 with one; from one of 50001: 80 and 81; 10^6 rows of 512 bytes from 32000: 138 and 158.  Lookups
+    // alone: 49 and 46, 60 and 59, 94 and 105), else as many waves as there are (32768 rows of 2 KB, alone: 15.6
+    // us, 16.7 with four)
     if (N * lpr >= (1LL << 22)) go(dt, std::integral_constant<int, 4>());
     else go(dt, std::integral_constant<int, 1>());
   };
@@ -626,7 +628,7 @@ extern "C" int s2c_embed_fwd(long long N, int V, int D, int dtype, long long ld,
 }
 
 // Looking through the tokens is one launch; where a word has many places its wave reads them alone, so
-// only few tokens (256 tokens, 3500 words of 300 columns: 4.3 us; the sort's three launches: 20 us).
+// only few tokens (256 tokens, 3500 words of 300 columns: 4.5 us; the sort's three launches: 15.4 us).
 static bool by_scan(long long N, int V) { return N <= STAGE && N * V <= (1LL << 26); }
 
 static long long align16(long long n) { return (n + 15) & ~15LL; }
@@ -634,7 +636,7 @@ static long long align16(long long n) { return (n + 15) & ~15LL; }
 static int pieces_of(int D, int vec) { return (D + 64 * vec - 1) / (64 * vec); }
 
 // About 4096 waves, and 64 places (a lane each) at most: shorter chunks leave more partial sums (131072
-// rows of 1024 bf16: runs 95 + join 25 us, 105 + 26 us with twice the waves).
+// rows of 1024 bf16: runs 82 + join 10 us, 98 + 12 us with twice the waves).
 static int chunk_of(long long N, int D) {
   const long long want = N * pieces_of(D, 8) / 4096;
   return want >= 64 ? 64 : want >= 32 ? 32 : want >= 16 ? 16 : 8;

@@ -19,11 +19,11 @@
 // walks its tiles in index order.
 //
 // All of it is bound by reading the logits and, backward, reading them again and writing the gradient; a
-// copy of 1 GiB reaches 5.1 TB/s here.  Kernel times on MI355X: 59392 x 3500 fp32 with 5 alternatives 157 us
-// (5.3 TB/s); 4096 x 50001 bf16 with 8 alternatives, a tenth of the rows ignored, 85 us forward (4.3 TB/s:
-// about half of it is the VALU's, 8 instructions an element) and 128 us backward; distillation over
-// 4096 x 65536 bf16 with 64 slots 116 us and 183 us (5.9 TB/s); one row of 32768 bf16 words 7.4 us (a launch,
-// a trip to memory and the selection's chain of ballots).
+// copy of 1 GiB reaches 5.1 TB/s here.  Kernel times on MI355X: 59392 x 3500 fp32 with 5 alternatives 158 us
+// (5.3 TB/s; 151 where nothing else runs between); 4096 x 50001 bf16 with 8 alternatives, a tenth of the rows
+// ignored, 85 to 88 us forward (4.3 TB/s: about half of it is the VALU's, 8 instructions an element) and 126 us
+// backward; distillation over 4096 x 65536 bf16 with 64 slots 115 us and 186 us (5.8 TB/s); one row of 32768 bf16
+// words 7.4 us (a launch, a trip to memory and the selection's chain of ballots).
 #include "s2c_words_common.h"
 
 #include <stdio.h>
@@ -248,9 +248,9 @@ __device__ __forceinline__ void stream_tile(const char *xr, int V, int shift, in
     const bool enter = __ballot(!(tmax <= thr)) != 0;
     if (enter && G > 1) {
       // few rows: what passes is rare and the code's length counts -- a mask of every lane's elements, then
-      // one of each lane at a time, read again (512 rows of 32000 words, 8 alternatives: 13.7 us, 14.7 with the
+      // one of each lane at a time, read again (512 rows of 32000 words, 8 alternatives: 13.4 us, 14.1 with the
       // elements unrolled as below).  A wave of its own per row meets more of them (59392 rows of 3500, 5
-      // alternatives: 161 us unrolled, 263 us when masks were tried there).
+      // alternatives: 150 us unrolled, 155 to 161 with masks).
       u32 hits = 0;
 #pragma unroll
       for (int u = 0; u < U; ++u)
@@ -858,14 +858,14 @@ long long vectors(int V, int dtype) {                  // of a row, at any align
 
 // How a row is shared out: `waves` of a workgroup to a stretch, `split` stretches to a row.
 //  * many rows: a wave each -- no barrier, no merge, one threshold for the whole row (59392 rows of 3500
-//    fp32 words, 5 alternatives: 157 us; 161 before its row lived in scalar registers, against 292 with
-//    4 waves a row);
-//  * rows that would leave most of the chip empty: 16 waves (32768 bf16 words, one row: 8.0 us, 9.7 with 4,
-//    20.9 with 1), and stretches of at least one round of tiles, up to 256 workgroups, joined by a second
-//    launch (64 rows of 131072 words: 17.4 us in 4 stretches, 18.6 in one; one row of 262144 fp32 words: 14.2
-//    in 16, 25.5 in one);
-//  * 4 waves between (512 rows of 32000 words: 15.5 us, 34.4 with 1, 20.4 with 16) and for short rows (248
-//    rows of 3500: 5.1 us, 5.3 with 16).
+//    fp32 words, 5 alternatives: 151 us, 303 with 4 waves a row);
+//  * rows that would leave most of the chip empty: 16 waves (32768 bf16 words, one row: 7.4 us, 8.6 with 4,
+//    19.9 with 1), and stretches of at least one round of tiles, up to 256 workgroups, joined by a second
+//    launch (64 rows of 131072 words, 20 alternatives: 14.9 us in 4 stretches, 17.2 in one; one row of 262144
+//    fp32 words: 13 in 16, 25.5 in one);
+//  * 4 waves between (512 rows of 32000 words: 13.4 us with 8 alternatives, 31.5 with 1, 17.7 with 16; without
+//    alternatives 9.8, 18.0 and 12.2; the floor is 6.4) and for short rows (248 rows of 3500: 3.9 us, the same
+//    with 16).
 struct Plan { int waves, split; };
 
 Plan forward_plan(int rows, int V, int dtype) {
@@ -902,14 +902,14 @@ template <bool DISTILL>
 int backward(GradArgs &a, const char *what, hipStream_t st) {
   const long long nvec = vectors(a.lg.V, a.lg.dtype);
   // waves of their own for short rows, whose stretches would leave most of a workgroup idle (59392 x 3500 bf16,
-  // 439 vectors: 154 us, 277 with 4 waves; 8192 x 8000, 1001 vectors: 48.5 and 45 us), and further where a
-  // stretch waits for its slots (the same with 32 slots: 52 and 56 us; 1000 x 10007, 33 slots: 13.4 and 17.7;
-  // 4096 x 65536, 64 slots: 206 and 182)
+  // 439 vectors: 156 us, 252 with 4 waves; 8192 x 8000, 1001 vectors: 47 and 44 us), and further where a
+  // stretch waits for its slots (the same with 32 slots: 51 and 55 us; 1000 x 10007, 33 slots: 13.0 and 16.7;
+  // 4096 x 65536, 64 slots: 198 and 184)
   const int G = nvec <= (DISTILL ? 2048 : 512) ? 1 : 4;
   a.segs = (int)((nvec + 64 * G * U - 1) / (64 * G * U));
   a.span = (int)((nvec + a.segs - 1) / a.segs);
   // a gradient that the 256 MB cache cannot hold would leave it full of lines to be written back: the
-  // next forward pass over 4096 x 50001 bf16 takes 122 us behind ordinary stores, 90 us behind these
+  // next forward pass over 4096 x 50001 bf16 takes 118 us behind ordinary stores, 82 to 90 us behind these
   a.past_cache = (double)a.lg.rows * a.lg.V * (a.lg.dtype == S2C_F32 ? 4 : 2) >= 256.0 * (1 << 20);
   const long long units = (long long)a.lg.rows * a.segs;
   by_type(a.lg.dtype, [&](auto dt) {
